@@ -413,6 +413,140 @@ spt_status spt_mul_q40_matrix(spt_context *ctx, spt_q40_matrix *m, const float *
 spt_status spt_mul_q40_matrix_device(spt_context *ctx, spt_q40_matrix *m, const float *x, float *y,
                                      int64_t batch);
 
+/* ---- 4-bit KV cache and attention over it ------------------------------------
+ * What stands between a layer's Q/K/V projections and its O projection
+ * (forward/attention.go:59-160 keeps an fp32 cache on the host): keys and
+ * values quantised as they are written, read back, and attended to.
+ *
+ * Format: 32 consecutive dims of one head of one token share a float16 scale
+ * d = m / -8, m being the block's element of largest magnitude (the first
+ * among equals), saturated to +-65504; a value x is held as
+ * n = clamp(round_half_even(x / d), -8, 7) and stands for n * d.  A block with
+ * a NaN stands for NaNs.  4.5 bits a value.
+ *
+ * A cache holds `pages` pages of `page_tokens` tokens on every layer; which
+ * page holds which tokens of which sequence is the caller's table.  A new
+ * cache is zero.  Calls that use one cache are enqueued on its context's
+ * stream; they share the cache's workspace, so calls that could overlap on
+ * the GPU (graphs replayed on two streams, a stream change without a wait
+ * between) have to be serialised by the caller. */
+typedef struct spt_kv_config {
+  int64_t layers;
+  int64_t kv_heads;
+  int64_t head_dim;    /* 32, 64, 96 or 128 */
+  int64_t page_tokens; /* a multiple of 16, at most 65536 */
+  int64_t pages;       /* at most 2^31 - 1 */
+} spt_kv_config;
+typedef struct spt_kv_cache spt_kv_cache;
+spt_status spt_kv_cache_create(spt_context *ctx, const spt_kv_config *cfg, spt_kv_cache **out);
+void spt_kv_cache_destroy(spt_kv_cache *cache); /* before its context's */
+uint64_t spt_kv_cache_bytes(const spt_kv_cache *cache);
+/* Checks a configuration without a device. */
+spt_status spt_kv_validate(spt_context *ctx, const spt_kv_config *cfg);
+
+/* The rows of a call.  Sequence b's new rows are offsets[b] .. offsets[b+1] - 1
+ * of the row arrays (offsets NULL: row b alone), and their positions are the
+ * last of its lengths[b] tokens; token p lies in page
+ * table[b * max_pages + p / page_tokens].  Rows of no sequence (a padded
+ * batch's tail) are neither read nor written.  Host calls take host arrays and
+ * refuse what does not fit; device calls take device arrays, which are not
+ * read on the host: there a row whose position or page lies outside the table
+ * or the pool is skipped, and keys on such pages are not attended to. */
+typedef struct spt_kv_rows {
+  int64_t sequences;
+  int64_t tokens;    /* rows of the row arrays */
+  int64_t max_pages; /* entries of a table row */
+  const int32_t *table;
+  const int32_t *lengths;
+  const int32_t *offsets;
+} spt_kv_rows;
+/* Types of rows: 0 F32, 1 F16, 30 BF16 (GGML numbers).  Strides are elements
+ * from row to row (0: rows without gaps); head h of a row starts at
+ * h * head_dim. */
+
+/* New rows of k and v into layer `layer`.  No two of them may fall on the same
+ * place of the same page: pages that sequences share are for reading. */
+spt_status spt_kv_append_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                                int32_t type, const void *k, int64_t k_stride, const void *v, int64_t v_stride);
+/* The same rows as the cache holds them (k or v may be NULL). */
+spt_status spt_kv_read_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                              int32_t type, void *k, int64_t k_stride, void *v, int64_t v_stride);
+
+/* Attention of every new row, at position p of its sequence, to the keys
+ * max(0, p - window + 1) .. p of the key head that its head belongs to
+ * (heads / kv_heads query heads share one):
+ *   s_j = scale * q . k_j
+ *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[head]))
+ * without the sink term where sinks is NULL.  A row without keys is 0.  A row
+ * of q with a NaN or an infinity gives NaNs and touches no other row.  The
+ * sums are held in 32 bits; f32 rows are multiplied as two float16 terms (22
+ * bits), so that the result is as good as 32-bit products'. */
+typedef struct spt_attention_config {
+  int64_t heads;      /* query heads, a multiple of kv_heads */
+  int64_t window;     /* keys a row sees at most; 0: all */
+  float scale;        /* positive */
+  const float *sinks; /* [heads] or NULL (device pointer in device calls) */
+} spt_attention_config;
+spt_status spt_attention_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                                const spt_attention_config *cfg, int32_t type, const void *q, int64_t q_stride,
+                                void *out, int64_t out_stride);
+/* Host arrays of fp32 rows without gaps, synchronous; lengths are element counts. */
+spt_status spt_kv_append(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                         const float *k, int64_t k_len, const float *v, int64_t v_len,
+                         const volatile int32_t *cancel);
+spt_status spt_kv_read(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows, float *k,
+                       int64_t k_len, float *v, int64_t v_len, const volatile int32_t *cancel);
+spt_status spt_attention(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                         const spt_attention_config *cfg, const float *q, int64_t q_len, float *out,
+                         int64_t out_len, const volatile int32_t *cancel);
+
+/* ---- Beam search -----------------------------------------------------------------
+ * Beside spt_mul_q80_matrix's argmax: the `keep` best continuations of each of
+ * `batch` searches of `beams` beams over the whole vocabulary,
+ *   score(j, t) = scores[j] + logits[j][t] - log sum_u exp(logits[j][u]),
+ * best first, equal scores in the order of beam and token.  A finished beam
+ * (finished may be NULL) offers end_token alone, with its score unchanged.  A
+ * NaN logit is no token, a score that is NaN or -inf (an unused beam's) no
+ * candidate; places without one get score -inf, parent -1, token -1.  The
+ * handle keeps the workspace of one call: its calls have to be serialised. */
+typedef struct spt_beam_config {
+  int64_t batch;
+  int64_t beams; /* at most 64; batch * beams at most 65535 */
+  int64_t vocab;
+  int64_t keep;  /* at most 64 */
+} spt_beam_config;
+typedef struct spt_beam spt_beam;
+spt_status spt_beam_validate(spt_context *ctx, const spt_beam_config *cfg);
+spt_status spt_beam_create(spt_context *ctx, const spt_beam_config *cfg, spt_beam **out);
+void spt_beam_destroy(spt_beam *beam); /* before its context's */
+/* logits [batch * beams] rows of `type`, row_stride elements apart (0: vocab);
+ * scores [batch][beams]; results [batch][keep]. */
+spt_status spt_beam_select_device(spt_context *ctx, spt_beam *beam, int32_t type, const void *logits,
+                                  int64_t row_stride, const float *scores, const uint8_t *finished,
+                                  int64_t end_token, float *out_scores, int32_t *out_parents,
+                                  int32_t *out_tokens);
+spt_status spt_beam_select(spt_context *ctx, spt_beam *beam, const float *logits, int64_t logits_len,
+                           const float *scores, const uint8_t *finished, int64_t end_token, float *out_scores,
+                           int32_t *out_parents, int32_t *out_tokens);
+/* Puts a cache's sequences (batch * beams of them, beam j of search b being
+ * sequence b * beams + j) in the order of their parents: sequence j continues
+ * parents[b * parents_stride + j].  It takes its parent's whole pages by
+ * number; a partial last page goes to the parent's first child, and every
+ * later child gets a copy, on all layers, in its own page spare[j].  Spare
+ * pages are distinct and in no table.  A parent outside [0, beams) leaves an
+ * empty sequence.  table_out (entries behind the last page -1), lengths_out
+ * and copied (1 where the spare page was taken; may be NULL) do not overlap
+ * the inputs.  Device pointers; pages outside the pool are not copied. */
+spt_status spt_kv_reorder_device(spt_context *ctx, spt_kv_cache *cache, int64_t batch, int64_t beams,
+                                 int64_t max_pages, const int32_t *parents, int64_t parents_stride,
+                                 const int32_t *table, const int32_t *lengths, const int32_t *spare,
+                                 int32_t *table_out, int32_t *lengths_out, uint8_t *copied);
+/* Host arrays, synchronous. */
+spt_status spt_kv_reorder(spt_context *ctx, spt_kv_cache *cache, int64_t batch, int64_t beams, int64_t max_pages,
+                          const int32_t *parents, int64_t parents_stride, const int32_t *table,
+                          const int32_t *lengths, const int32_t *spare, int32_t *table_out, int32_t *lengths_out,
+                          uint8_t *copied);
+
 /* ---- GGUF model files -------------------------------------------------------
  * ggufindex.Open (ggufindex/index.go:55-575): headers, metadata and tensor
  * directories of one model, split files in any order, each file mapped

@@ -83,6 +83,24 @@ class _SynthParams(ctypes.Structure):
                 ("zipf_beta", ctypes.c_float)]
 
 
+class _KvConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("layers", "kv_heads", "head_dim", "page_tokens", "pages")]
+
+
+class _KvRows(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("sequences", "tokens", "max_pages")] + \
+               [(n, ctypes.c_void_p) for n in ("table", "lengths", "offsets")]
+
+
+class _AttentionConfig(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_int64), ("window", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("sinks", ctypes.c_void_p)]
+
+
+class _BeamConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "beams", "vocab", "keep")]
+
+
 # ---- Go-side value types ---------------------------------------------------
 @dataclass
 class Tensor:
@@ -240,6 +258,23 @@ def lib():
         "spt_q80_matrix_destroy": ([vp], None),
         "spt_mul_q80_matrix": ([vp, vp, vp, vp, P(i64), P(f32)], st),
         "spt_mul_q80_matrix_device": ([vp, vp, vp, vp, vp, vp], st),
+        "spt_kv_validate": ([vp, P(_KvConfig)], st),
+        "spt_kv_cache_create": ([vp, P(_KvConfig), P(vp)], st),
+        "spt_kv_cache_destroy": ([vp], None),
+        "spt_kv_cache_bytes": ([vp], ctypes.c_uint64),
+        "spt_kv_append_device": ([vp, vp, i64, P(_KvRows), i32, vp, i64, vp, i64], st),
+        "spt_kv_read_device": ([vp, vp, i64, P(_KvRows), i32, vp, i64, vp, i64], st),
+        "spt_attention_device": ([vp, vp, i64, P(_KvRows), P(_AttentionConfig), i32, vp, i64, vp, i64], st),
+        "spt_kv_append": ([vp, vp, i64, P(_KvRows), vp, i64, vp, i64, vp], st),
+        "spt_kv_read": ([vp, vp, i64, P(_KvRows), vp, i64, vp, i64, vp], st),
+        "spt_attention": ([vp, vp, i64, P(_KvRows), P(_AttentionConfig), vp, i64, vp, i64, vp], st),
+        "spt_beam_validate": ([vp, P(_BeamConfig)], st),
+        "spt_beam_create": ([vp, P(_BeamConfig), P(vp)], st),
+        "spt_beam_destroy": ([vp], None),
+        "spt_beam_select_device": ([vp, vp, i32, vp, i64, vp, vp, i64, vp, vp, vp], st),
+        "spt_beam_select": ([vp, vp, vp, i64, vp, vp, i64, vp, vp, vp], st),
+        "spt_kv_reorder_device": ([vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp], st),
+        "spt_kv_reorder": ([vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp], st),
         "spt_ep_expert_range": ([i64, i32, i32, P(i64), P(i64)], None),
         "spt_last_dispatch": ([vp, P(i64), P(i64)], st),
         "spt_ep_unique_id": ([vp], st),
@@ -623,6 +658,25 @@ class Context:
         """Upload a Q4_0 tensor once (spt_q40_matrix_create)."""
         return Q40Matrix(self, reader, tensor)
 
+    # ---- 4-bit KV cache, beam search ----------------------------------------
+    def kv_cache(self, kv_heads: int, head_dim: int, page_tokens: int, pages: int, layers: int = 1) -> "KvCache":
+        """A zeroed 4-bit KV cache (spt_kv_cache_create)."""
+        return KvCache(self, kv_heads, head_dim, page_tokens, pages, layers)
+
+    def validate_kv(self, kv_heads: int, head_dim: int, page_tokens: int, pages: int, layers: int = 1):
+        """spt_kv_cache_create's checks, without a device."""
+        c = _KvConfig(layers, kv_heads, head_dim, page_tokens, pages)
+        self.check(lib().spt_kv_validate(self._h, ctypes.byref(c)))
+
+    def beam(self, batch: int, beams: int, vocab: int, keep: int) -> "Beam":
+        """Beam selection for `batch` searches of `beams` beams (spt_beam_create)."""
+        return Beam(self, batch, beams, vocab, keep)
+
+    def validate_beam(self, batch: int, beams: int, vocab: int, keep: int):
+        """spt_beam_create's checks, without a device."""
+        c = _BeamConfig(batch, beams, vocab, keep)
+        self.check(lib().spt_beam_validate(self._h, ctypes.byref(c)))
+
     def q80_matrix(self, data: np.ndarray, input_: int, output: int) -> "Q80Matrix":
         """Upload a Q8_0 matrix once (spt_q80_matrix_create)."""
         return Q80Matrix(self, data, input_, output)
@@ -755,6 +809,159 @@ class Q80Matrix:
         if self._h:
             lib().spt_q80_matrix_destroy(self._h)
             self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvBatch:
+    """spt_kv_rows: which rows of a call belong to which sequence, and where
+    their tokens lie.  `table` [sequences, max_pages], `lengths` [sequences]
+    and `offsets` [sequences + 1] (None or 0: row b is sequence b's one new
+    row) are device addresses for the *_device calls, or int32 arrays for the
+    host calls."""
+
+    def __init__(self, sequences: int, tokens: int, max_pages: int, table, lengths, offsets=None):
+        self._keep = []
+
+        def address(a):
+            if a is None or isinstance(a, int):
+                return a or None
+            a = np.ascontiguousarray(a, dtype=np.int32)
+            self._keep.append(a)
+            return a.ctypes.data
+
+        self.c = _KvRows(sequences, tokens, max_pages, address(table), address(lengths), address(offsets))
+        self.tokens = tokens
+        self.ref = ctypes.byref(self.c)
+
+
+class KvCache:
+    """4-bit KV cache (spt_kv_cache): append, read back, attend, reorder."""
+
+    def __init__(self, ctx: "Context", kv_heads: int, head_dim: int, page_tokens: int, pages: int, layers: int = 1):
+        self.ctx, self.kv_heads, self.head_dim = ctx, kv_heads, head_dim
+        self.page_tokens, self.pages, self.layers = page_tokens, pages, layers
+        self._h = ctypes.c_void_p()
+        c = _KvConfig(layers, kv_heads, head_dim, page_tokens, pages)
+        ctx.check(lib().spt_kv_cache_create(ctx._h, ctypes.byref(c), ctypes.byref(self._h)))
+
+    @property
+    def nbytes(self) -> int:
+        return int(lib().spt_kv_cache_bytes(self._h))
+
+    def append_device(self, batch: KvBatch, k_ptr: int, v_ptr: int, type: int = GGML_F32, layer: int = 0,
+                      k_stride: int = 0, v_stride: int = 0):
+        self.ctx.check(lib().spt_kv_append_device(self.ctx._h, self._h, layer, batch.ref, type, k_ptr, k_stride, v_ptr,
+                                                  v_stride))
+
+    def read_device(self, batch: KvBatch, k_ptr: int, v_ptr: int, type: int = GGML_F32, layer: int = 0,
+                    k_stride: int = 0, v_stride: int = 0):
+        self.ctx.check(lib().spt_kv_read_device(self.ctx._h, self._h, layer, batch.ref, type, k_ptr or None, k_stride,
+                                                v_ptr or None, v_stride))
+
+    def attention_device(self, batch: KvBatch, q_ptr: int, out_ptr: int, heads: int, type: int = GGML_F32,
+                         scale: float = 1.0, window: int = 0, sinks_ptr: int = 0, layer: int = 0, q_stride: int = 0,
+                         out_stride: int = 0):
+        c = _AttentionConfig(heads, window, scale, sinks_ptr or None)
+        self.ctx.check(lib().spt_attention_device(self.ctx._h, self._h, layer, batch.ref, ctypes.byref(c), type, q_ptr,
+                                                  q_stride, out_ptr, out_stride))
+
+    def append(self, batch: KvBatch, k: np.ndarray, v: np.ndarray, layer: int = 0, cancel=None):
+        k, v = _f32(k), _f32(v)
+        self.ctx.check(lib().spt_kv_append(self.ctx._h, self._h, layer, batch.ref, _p(k), k.size, _p(v), v.size,
+                                           _p(cancel)))
+
+    def read(self, batch: KvBatch, layer: int = 0, cancel=None):
+        """(k, v) [tokens, kv_heads, head_dim] as the cache holds them (0 in rows of no sequence)."""
+        shape = (batch.tokens, self.kv_heads, self.head_dim)
+        k, v = np.zeros(shape, np.float32), np.zeros(shape, np.float32)
+        self.ctx.check(lib().spt_kv_read(self.ctx._h, self._h, layer, batch.ref, _p(k), k.size, _p(v), v.size,
+                                         _p(cancel)))
+        return k, v
+
+    def attention(self, batch: KvBatch, q: np.ndarray, heads: int, scale: float = 1.0, window: int = 0,
+                  sinks: Optional[np.ndarray] = None, layer: int = 0, out: Optional[np.ndarray] = None,
+                  cancel=None) -> np.ndarray:
+        """[tokens, heads, head_dim]; rows of no sequence stay as `out` has them (0 without `out`)."""
+        q = _f32(q)
+        sinks = None if sinks is None else _f32(sinks)
+        if out is None:
+            out = np.zeros((batch.tokens, heads, self.head_dim), np.float32)
+        c = _AttentionConfig(heads, window, scale, None if sinks is None else sinks.ctypes.data)
+        self.ctx.check(lib().spt_attention(self.ctx._h, self._h, layer, batch.ref, ctypes.byref(c), _p(q), q.size,
+                                           _p(out), out.size, _p(cancel)))
+        return out
+
+    def reorder_device(self, batch: int, beams: int, max_pages: int, parents_ptr: int, parents_stride: int,
+                       table_ptr: int, lengths_ptr: int, spare_ptr: int, table_out_ptr: int, lengths_out_ptr: int,
+                       copied_ptr: int = 0):
+        self.ctx.check(lib().spt_kv_reorder_device(self.ctx._h, self._h, batch, beams, max_pages, parents_ptr,
+                                                   parents_stride, table_ptr, lengths_ptr, spare_ptr, table_out_ptr,
+                                                   lengths_out_ptr, copied_ptr or None))
+
+    def reorder(self, parents: np.ndarray, table: np.ndarray, lengths: np.ndarray, spare: np.ndarray):
+        """(table, lengths, copied) after each sequence [batch, beams] has taken its parent's place."""
+        parents = np.ascontiguousarray(parents, dtype=np.int32)
+        batch, beams = parents.shape
+        table = np.ascontiguousarray(table, dtype=np.int32)
+        lengths = np.ascontiguousarray(lengths, dtype=np.int32)
+        spare = np.ascontiguousarray(spare, dtype=np.int32)
+        new_table, new_lengths = np.empty_like(table), np.empty_like(lengths)
+        copied = np.empty(batch * beams, np.uint8)
+        self.ctx.check(lib().spt_kv_reorder(self.ctx._h, self._h, batch, beams, table.shape[-1], _p(parents), beams,
+                                            _p(table), _p(lengths), _p(spare), _p(new_table), _p(new_lengths),
+                                            _p(copied)))
+        return new_table, new_lengths, copied
+
+    def close(self):
+        if self._h and self.ctx._h:  # a closed context took its stream along
+            lib().spt_kv_cache_destroy(self._h)
+        self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Beam:
+    """Beam search's selection (spt_beam): the `keep` best continuations of each search."""
+
+    def __init__(self, ctx: "Context", batch: int, beams: int, vocab: int, keep: int):
+        self.ctx, self.batch, self.beams, self.vocab, self.keep = ctx, batch, beams, vocab, keep
+        self._h = ctypes.c_void_p()
+        c = _BeamConfig(batch, beams, vocab, keep)
+        ctx.check(lib().spt_beam_create(ctx._h, ctypes.byref(c), ctypes.byref(self._h)))
+
+    def select_device(self, logits_ptr: int, scores_ptr: int, out_scores_ptr: int, out_parents_ptr: int,
+                      out_tokens_ptr: int, type: int = GGML_F32, row_stride: int = 0, finished_ptr: int = 0,
+                      end_token: int = 0):
+        self.ctx.check(lib().spt_beam_select_device(self.ctx._h, self._h, type, logits_ptr, row_stride, scores_ptr,
+                                                    finished_ptr or None, end_token, out_scores_ptr, out_parents_ptr,
+                                                    out_tokens_ptr))
+
+    def select(self, logits: np.ndarray, scores: np.ndarray, finished: Optional[np.ndarray] = None,
+               end_token: int = 0):
+        """(scores, parents, tokens), each [batch, keep], best first."""
+        logits, scores = _f32(logits), _f32(scores)
+        finished = None if finished is None else np.ascontiguousarray(finished, dtype=np.uint8)
+        if scores.size != self.batch * self.beams or (finished is not None and finished.size != scores.size):
+            raise SptError(ERR_DIMENSIONS, f"expected {self.batch * self.beams} beam scores and flags")
+        shape = (self.batch, self.keep)
+        out, parents, tokens = np.empty(shape, np.float32), np.empty(shape, np.int32), np.empty(shape, np.int32)
+        self.ctx.check(lib().spt_beam_select(self.ctx._h, self._h, _p(logits), logits.size, _p(scores), _p(finished),
+                                             end_token, _p(out), _p(parents), _p(tokens)))
+        return out, parents, tokens
+
+    def close(self):
+        if self._h and self.ctx._h:  # a closed context took its stream along
+            lib().spt_beam_destroy(self._h)
+        self._h = ctypes.c_void_p()
 
     def __del__(self):
         try:

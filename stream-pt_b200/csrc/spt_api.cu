@@ -17,12 +17,14 @@
 #include <initializer_list>
 #include <limits>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/spt_moe.h"
 #include "spt_gguf.h"
 #include "spt_internal.cuh"
+#include "spt_kv.cuh"
 #include "spt_philox.h"
 
 using namespace spt;
@@ -3436,6 +3438,600 @@ spt_status spt_arena_create_gguf(spt_context *ctx, const spt_gguf *g, int64_t fi
       return fail(ctx, st, "%s", spt_last_error(nullptr));
   if (expert_end == 0) expert_end = cfg.num_experts;
   return arena_create_impl(ctx, readers.data(), &cfg, lws.data(), n_layers, flags, expert_begin, expert_end, out);
+}
+
+}  // extern "C"
+
+// =========================================================================
+// 4-bit KV cache, attention over it, beam search (spt_kv.cu, spt_attn.cu,
+// spt_beam.cu).
+struct spt_kv_cache {
+  spt_context *ctx = nullptr;
+  spt_kv_config cfg{};
+  DevBuf pool;              // [layers] x layer_bytes
+  int64_t layer_bytes = 0;
+  DevBuf partial, arrive;   // attention: parts of items that several CTAs share, and their arrivals (zero between launches)
+  DevBuf hin, hin2, hout, hint, hsmall;  // host calls' staging: rows, tables, sinks
+};
+
+struct spt_beam {
+  spt_context *ctx = nullptr;
+  spt_beam_config cfg{};
+  DevBuf work;
+  DevBuf hlogits, hsmall;   // host calls' staging
+};
+
+namespace {
+
+int type_size(int32_t type) { return type == kKvF32 ? 4 : type == kKvF16 || type == kKvBF16 ? 2 : 0; }
+
+bool aligned(const void *p, int size) { return ((uintptr_t)p & (uintptr_t)(size - 1)) == 0; }
+
+spt_status kv_config(spt_context *ctx, const spt_kv_config *c, int64_t *layer_bytes) {
+  if (!c) return fail(ctx, SPT_ERR_NULL_ARG, "nil KV cache configuration");
+  if (c->layers <= 0 || c->kv_heads <= 0 || c->pages <= 0 || c->page_tokens <= 0 || c->head_dim <= 0)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "invalid KV cache dimensions");
+  if (c->head_dim % 32 != 0 || c->head_dim > 32 * kKvMaxBlocks)
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "head dimension %lld instead of 32, 64, 96 or 128", (long long)c->head_dim);
+  if (c->page_tokens % kKvTile != 0 || c->page_tokens > 65536)
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "%lld tokens a page: a multiple of 16, at most 65536, is needed",
+                (long long)c->page_tokens);
+  if (c->pages > INT32_MAX || c->kv_heads > 4096 || c->layers > 65536)
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "KV cache dimensions exceed this build's limits");
+  int64_t bytes = 0;
+  if (!product({c->pages, c->kv_heads, c->page_tokens / kKvTile, kv_tile_bytes((int)(c->head_dim / 32))}, &bytes) ||
+      !product({bytes, c->layers}, nullptr))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "KV cache size overflows");
+  if (layer_bytes) *layer_bytes = bytes;
+  return SPT_OK;
+}
+
+KvLayer kv_layer(const spt_kv_cache *c, int64_t layer) {
+  KvLayer l;
+  l.base = c->pool.as<uint8_t>() + layer * c->layer_bytes;
+  l.pages = c->cfg.pages;
+  l.kv_heads = (int)c->cfg.kv_heads;
+  l.nb = (int)(c->cfg.head_dim / 32);
+  l.page_tokens = (int)c->cfg.page_tokens;
+  return l;
+}
+
+// Checks that need no look at the arrays' contents.
+spt_status kv_call(spt_context *ctx, const spt_kv_cache *cache, int64_t layer, const spt_kv_rows *r) {
+  if (!ctx || !cache || !r) return fail(ctx, SPT_ERR_NULL_ARG, "nil context, KV cache or rows");
+  if (cache->ctx != ctx) return fail(ctx, SPT_ERR_DIMENSIONS, "KV cache belongs to another context");
+  if (layer < 0 || layer >= cache->cfg.layers)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "layer %lld outside the KV cache's %lld", (long long)layer,
+                (long long)cache->cfg.layers);
+  if (r->sequences < 0 || r->tokens < 0 || r->max_pages < 0 || r->sequences > INT32_MAX || r->tokens > INT32_MAX ||
+      r->max_pages > INT32_MAX)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "invalid KV row counts");
+  if (r->sequences > 0 && (!r->lengths || (!r->table && r->max_pages > 0)))
+    return fail(ctx, SPT_ERR_NULL_ARG, "nil page table or lengths");
+  if (!aligned(r->table, 4) || !aligned(r->lengths, 4) || !aligned(r->offsets, 4))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "page table, lengths or offsets not aligned to 4 bytes");
+  return SPT_OK;
+}
+
+KvRows kv_rows(const spt_kv_rows *r) {
+  KvRows k;
+  k.table = r->table;
+  k.lengths = r->lengths;
+  k.offsets = r->offsets;
+  k.sequences = r->sequences;
+  k.tokens = r->tokens;
+  k.max_pages = r->max_pages;
+  return k;
+}
+
+// One row array: its type, alignment and stride (0: without gaps).
+spt_status row_array(spt_context *ctx, const void *p, int32_t type, int64_t width, int64_t tokens, int64_t *stride) {
+  const int size = type_size(type);
+  if (!size) return fail(ctx, SPT_ERR_UNSUPPORTED, "row type %d instead of F32 (0), F16 (1) or BF16 (30)", (int)type);
+  if (*stride == 0) *stride = width;
+  if (*stride < width) return fail(ctx, SPT_ERR_DIMENSIONS, "row stride %lld below the row's %lld elements",
+                                   (long long)*stride, (long long)width);
+  if (*stride > ((int64_t)1 << 40)) return fail(ctx, SPT_ERR_DIMENSIONS, "row stride %lld", (long long)*stride);
+  (void)tokens;
+  if (!aligned(p, size)) return fail(ctx, SPT_ERR_DIMENSIONS, "rows not aligned to their type");
+  return SPT_OK;
+}
+
+spt_status attention_config(spt_context *ctx, const spt_kv_cache *cache, const spt_attention_config *cfg) {
+  if (!cfg) return fail(ctx, SPT_ERR_NULL_ARG, "nil attention configuration");
+  if (cfg->heads <= 0 || cfg->heads % cache->cfg.kv_heads != 0 || cfg->heads > 65536)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "%lld query heads on %lld key heads", (long long)cfg->heads,
+                (long long)cache->cfg.kv_heads);
+  if (cfg->window < 0) return fail(ctx, SPT_ERR_DIMENSIONS, "window %lld", (long long)cfg->window);
+  if (!(cfg->scale > 0.0f) || !std::isfinite(cfg->scale))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "attention scale %g", (double)cfg->scale);
+  if (!aligned(cfg->sinks, 4)) return fail(ctx, SPT_ERR_DIMENSIONS, "sinks not aligned to 4 bytes");
+  return SPT_OK;
+}
+
+// The contents of a host call's arrays: every position has its page.
+spt_status kv_host_rows(spt_context *ctx, const spt_kv_cache *cache, const spt_kv_rows *r) {
+  const int64_t page = cache->cfg.page_tokens;
+  int64_t at = 0;
+  if (r->offsets && r->sequences > 0 && r->offsets[0] < 0) return fail(ctx, SPT_ERR_DIMENSIONS, "negative offset");
+  for (int64_t b = 0; b < r->sequences; ++b) {
+    const int64_t n = r->offsets ? (int64_t)r->offsets[b + 1] - r->offsets[b] : 1;
+    at = r->offsets ? r->offsets[b + 1] : b + 1;
+    if (n < 0 || at > r->tokens)
+      return fail(ctx, SPT_ERR_DIMENSIONS, "rows of sequence %lld outside the %lld given", (long long)b,
+                  (long long)r->tokens);
+    const int64_t len = r->lengths[b];
+    if (len < n) return fail(ctx, SPT_ERR_DIMENSIONS, "sequence %lld: %lld new rows but a length of %lld",
+                             (long long)b, (long long)n, (long long)len);
+    const int64_t used = (len + page - 1) / page;
+    if (used > r->max_pages)
+      return fail(ctx, SPT_ERR_DIMENSIONS, "sequence %lld: a length of %lld exceeds %lld pages", (long long)b,
+                  (long long)len, (long long)r->max_pages);
+    for (int64_t i = 0; i < used; ++i) {
+      const int64_t p = r->table[b * r->max_pages + i];
+      if (p < 0 || p >= cache->cfg.pages)
+        return fail(ctx, SPT_ERR_DIMENSIONS, "sequence %lld: page %lld outside the pool of %lld", (long long)b,
+                    (long long)p, (long long)cache->cfg.pages);
+    }
+  }
+  return SPT_OK;
+}
+
+// Host tables on the device, in the cache's staging buffer.
+spt_status kv_stage_rows(spt_context *ctx, spt_kv_cache *cache, const spt_kv_rows *r, spt_kv_rows *dev) {
+  const int64_t n_table = r->sequences * r->max_pages, n_off = r->offsets ? r->sequences + 1 : 0;
+  SPT_CUDA(ctx, cache->hint.ensure(sizeof(int32_t) * (size_t)(n_table + r->sequences + n_off)));
+  int32_t *d = cache->hint.as<int32_t>();
+  if (n_table)
+    SPT_CUDA(ctx, cudaMemcpyAsync(d, r->table, sizeof(int32_t) * n_table, cudaMemcpyHostToDevice, ctx->stream));
+  if (r->sequences)
+    SPT_CUDA(ctx, cudaMemcpyAsync(d + n_table, r->lengths, sizeof(int32_t) * r->sequences, cudaMemcpyHostToDevice,
+                                  ctx->stream));
+  if (n_off)
+    SPT_CUDA(ctx, cudaMemcpyAsync(d + n_table + r->sequences, r->offsets, sizeof(int32_t) * n_off,
+                                  cudaMemcpyHostToDevice, ctx->stream));
+  *dev = *r;
+  dev->table = d;
+  dev->lengths = d + n_table;
+  dev->offsets = n_off ? d + n_table + r->sequences : nullptr;
+  return SPT_OK;
+}
+
+bool ranges_overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+spt_status beam_config(spt_context *ctx, const spt_beam_config *c) {
+  if (!c) return fail(ctx, SPT_ERR_NULL_ARG, "nil beam configuration");
+  if (c->batch <= 0 || c->beams <= 0 || c->vocab <= 0 || c->keep <= 0)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "invalid beam search dimensions");
+  if (c->beams > kBeamMaxBeams || c->keep > kBeamMaxKeep || c->batch > 65535 / c->beams ||
+      c->vocab > INT32_MAX - (1 << 20))
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "beam search dimensions exceed this build's limits");
+  return SPT_OK;
+}
+
+spt_status reorder_args(spt_context *ctx, const spt_kv_cache *cache, int64_t batch, int64_t beams, int64_t max_pages,
+                        const int32_t *parents, int64_t parents_stride, const int32_t *table, const int32_t *lengths,
+                        const int32_t *spare, const int32_t *table_out, const int32_t *lengths_out,
+                        const uint8_t *copied) {
+  if (!ctx || !cache) return fail(ctx, SPT_ERR_NULL_ARG, "nil context or KV cache");
+  if (cache->ctx != ctx) return fail(ctx, SPT_ERR_DIMENSIONS, "KV cache belongs to another context");
+  int64_t n = 0;
+  if (batch <= 0 || beams <= 0 || max_pages <= 0 || parents_stride < beams || !product({batch, beams}, &n) ||
+      n > INT32_MAX || max_pages > INT32_MAX || parents_stride > INT32_MAX)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "invalid beam reorder dimensions");
+  if (beams > kBeamMaxBeams) return fail(ctx, SPT_ERR_UNSUPPORTED, "%lld beams", (long long)beams);
+  if (!parents || !table || !lengths || !spare || !table_out || !lengths_out)
+    return fail(ctx, SPT_ERR_NULL_ARG, "nil beam reorder array");
+  for (const int32_t *p : {parents, table, lengths, spare, table_out, lengths_out})
+    if (!aligned(p, 4)) return fail(ctx, SPT_ERR_DIMENSIONS, "beam reorder array not aligned to 4 bytes");
+  const struct { const void *p; int64_t n; } in[] = {{parents, ((batch - 1) * parents_stride + beams) * 4},
+                                                     {table, n * max_pages * 4}, {lengths, n * 4}, {spare, n * 4}},
+                                             out[] = {{table_out, n * max_pages * 4}, {lengths_out, n * 4},
+                                                      {copied, copied ? n : 0}};
+  for (int i = 0; i < 3; ++i) {
+    for (const auto &x : in)
+      if (ranges_overlap(x.p, x.n, out[i].p, out[i].n))
+        return fail(ctx, SPT_ERR_OVERLAP, "beam reorder inputs and outputs must not overlap");
+    for (int j = 0; j < i; ++j)
+      if (ranges_overlap(out[i].p, out[i].n, out[j].p, out[j].n))
+        return fail(ctx, SPT_ERR_OVERLAP, "beam reorder outputs must not overlap");
+  }
+  return SPT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+spt_status spt_kv_validate(spt_context *ctx, const spt_kv_config *cfg) {
+  if (!ctx) return fail(nullptr, SPT_ERR_NULL_ARG, "nil context");
+  return kv_config(ctx, cfg, nullptr);
+}
+
+spt_status spt_kv_cache_create(spt_context *ctx, const spt_kv_config *cfg, spt_kv_cache **out) {
+  if (!ctx || !out) return fail(ctx, SPT_ERR_NULL_ARG, "nil context or output");
+  *out = nullptr;
+  int64_t layer_bytes = 0;
+  spt_status st = kv_config(ctx, cfg, &layer_bytes);
+  if (st) return st;
+  if ((st = require_device(ctx))) return st;
+  spt_kv_cache *c = new (std::nothrow) spt_kv_cache();
+  if (!c) return fail(ctx, SPT_ERR_CUDA, "KV cache: out of host memory");
+  c->ctx = ctx;
+  c->cfg = *cfg;
+  c->layer_bytes = layer_bytes;
+  const size_t bytes = (size_t)layer_bytes * (size_t)cfg->layers;
+  cudaError_t e = c->pool.ensure(bytes);
+  if (e == cudaSuccess) e = cudaMemsetAsync(c->pool.p, 0, bytes, ctx->stream);
+  if (e == cudaSuccess) e = c->partial.ensure(attn_workspace_bytes(ctx->sm_count, (int)(cfg->head_dim / 32)));
+  if (e == cudaSuccess) e = c->arrive.ensure(attn_counter_bytes(ctx->sm_count));
+  if (e == cudaSuccess) e = cudaMemsetAsync(c->arrive.p, 0, c->arrive.bytes, ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    spt_kv_cache_destroy(c);
+    return cuda_fail(ctx, e, "KV cache allocation");
+  }
+  *out = c;
+  return SPT_OK;
+}
+
+void spt_kv_cache_destroy(spt_kv_cache *c) {
+  if (!c) return;
+  if (c->ctx && c->ctx->has_device) {
+    cudaSetDevice(c->ctx->device);
+    cudaStreamSynchronize(c->ctx->stream);
+  }
+  for (DevBuf *b : {&c->pool, &c->partial, &c->arrive, &c->hin, &c->hin2, &c->hout, &c->hint, &c->hsmall})
+    b->release();
+  delete c;
+}
+
+uint64_t spt_kv_cache_bytes(const spt_kv_cache *c) {
+  return c ? (uint64_t)c->layer_bytes * (uint64_t)c->cfg.layers : 0;
+}
+
+spt_status spt_kv_append_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                                int32_t type, const void *k, int64_t k_stride, const void *v, int64_t v_stride) {
+  spt_status st = kv_call(ctx, cache, layer, rows);
+  if (st) return st;
+  const int64_t width = cache->cfg.kv_heads * cache->cfg.head_dim;
+  if ((st = row_array(ctx, k, type, width, rows->tokens, &k_stride))) return st;
+  if ((st = row_array(ctx, v, type, width, rows->tokens, &v_stride))) return st;
+  if (rows->tokens > 0 && (!k || !v)) return fail(ctx, SPT_ERR_NULL_ARG, "nil key or value rows");
+  if ((st = require_device(ctx))) return st;
+  SPT_CUDA(ctx, launch_kv_append(kv_layer(cache, layer), kv_rows(rows), type, k, k_stride, v, v_stride, ctx->stream));
+  ctx->kernels_last = 1;
+  return SPT_OK;
+}
+
+spt_status spt_kv_read_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                              int32_t type, void *k, int64_t k_stride, void *v, int64_t v_stride) {
+  spt_status st = kv_call(ctx, cache, layer, rows);
+  if (st) return st;
+  const int64_t width = cache->cfg.kv_heads * cache->cfg.head_dim;
+  if ((st = row_array(ctx, k, type, width, rows->tokens, &k_stride))) return st;
+  if ((st = row_array(ctx, v, type, width, rows->tokens, &v_stride))) return st;
+  if ((st = require_device(ctx))) return st;
+  if (!k && !v) return SPT_OK;
+  SPT_CUDA(ctx, launch_kv_read(kv_layer(cache, layer), kv_rows(rows), type, k, k_stride, v, v_stride, ctx->stream));
+  ctx->kernels_last = 1;
+  return SPT_OK;
+}
+
+spt_status spt_attention_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                                const spt_attention_config *cfg, int32_t type, const void *q, int64_t q_stride,
+                                void *out, int64_t out_stride) {
+  spt_status st = kv_call(ctx, cache, layer, rows);
+  if (st) return st;
+  if ((st = attention_config(ctx, cache, cfg))) return st;
+  const int64_t width = cfg->heads * cache->cfg.head_dim;
+  if ((st = row_array(ctx, q, type, width, rows->tokens, &q_stride))) return st;
+  if ((st = row_array(ctx, out, type, width, rows->tokens, &out_stride))) return st;
+  if (rows->tokens > 0) {
+    if (!q || !out) return fail(ctx, SPT_ERR_NULL_ARG, "nil query or output rows");
+    const int size = type_size(type);
+    if (ranges_overlap(q, ((rows->tokens - 1) * q_stride + width) * size, out,
+                       ((rows->tokens - 1) * out_stride + width) * size))
+      return fail(ctx, SPT_ERR_OVERLAP, "query and output rows must not overlap");
+  }
+  if ((st = require_device(ctx))) return st;
+  AttnArgs a;
+  a.c = kv_layer(cache, layer);
+  a.r = kv_rows(rows);
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.sinks = cfg->sinks;
+  a.scale = cfg->scale;
+  a.window = cfg->window;
+  a.heads = (int)cfg->heads;
+  a.group = (int)(cfg->heads / cache->cfg.kv_heads);
+  a.type = type;
+  a.partial = cache->partial.as<float>();
+  a.arrive = cache->arrive.as<int32_t>();
+  a.sm_count = ctx->sm_count;
+  SPT_CUDA(ctx, launch_attention(a, ctx->stream));
+  ctx->kernels_last = 1;
+  return SPT_OK;
+}
+
+spt_status spt_kv_append(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                         const float *k, int64_t k_len, const float *v, int64_t v_len,
+                         const volatile int32_t *cancel) {
+  spt_status st = kv_call(ctx, cache, layer, rows);
+  if (st) return st;
+  const int64_t n = rows->tokens * cache->cfg.kv_heads * cache->cfg.head_dim;
+  if (k_len != n || v_len != n)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "expected %lld key and value elements, got %lld and %lld", (long long)n,
+                (long long)k_len, (long long)v_len);
+  if (n > 0 && (!k || !v)) return fail(ctx, SPT_ERR_NULL_ARG, "nil key or value rows");
+  if ((st = kv_host_rows(ctx, cache, rows))) return st;
+  if (canceled(cancel)) return fail(ctx, SPT_ERR_CANCELED, "context canceled");
+  if ((st = require_device(ctx))) return st;
+  if (n == 0) return SPT_OK;
+  spt_kv_rows dev;
+  if ((st = kv_stage_rows(ctx, cache, rows, &dev))) return st;
+  const size_t bytes = sizeof(float) * (size_t)n;
+  SPT_CUDA(ctx, cache->hin.ensure(bytes));
+  SPT_CUDA(ctx, cache->hin2.ensure(bytes));
+  SPT_CUDA(ctx, cudaMemcpyAsync(cache->hin.p, k, bytes, cudaMemcpyHostToDevice, ctx->stream));
+  SPT_CUDA(ctx, cudaMemcpyAsync(cache->hin2.p, v, bytes, cudaMemcpyHostToDevice, ctx->stream));
+  if ((st = spt_kv_append_device(ctx, cache, layer, &dev, kKvF32, cache->hin.p, 0, cache->hin2.p, 0))) return st;
+  SPT_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  return SPT_OK;
+}
+
+spt_status spt_kv_read(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows, float *k,
+                       int64_t k_len, float *v, int64_t v_len, const volatile int32_t *cancel) {
+  spt_status st = kv_call(ctx, cache, layer, rows);
+  if (st) return st;
+  const int64_t n = rows->tokens * cache->cfg.kv_heads * cache->cfg.head_dim;
+  if ((k && k_len != n) || (v && v_len != n))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "expected %lld key and value elements, got %lld and %lld", (long long)n,
+                (long long)k_len, (long long)v_len);
+  if ((st = kv_host_rows(ctx, cache, rows))) return st;
+  if (canceled(cancel)) return fail(ctx, SPT_ERR_CANCELED, "context canceled");
+  if ((st = require_device(ctx))) return st;
+  if (n == 0 || (!k && !v)) return SPT_OK;
+  spt_kv_rows dev;
+  if ((st = kv_stage_rows(ctx, cache, rows, &dev))) return st;
+  const size_t bytes = sizeof(float) * (size_t)n;
+  float *host[2] = {k, v};
+  DevBuf *buf[2] = {&cache->hin, &cache->hin2};
+  for (int i = 0; i < 2; ++i) {  // rows of no sequence come back as they were
+    if (!host[i]) continue;
+    SPT_CUDA(ctx, buf[i]->ensure(bytes));
+    SPT_CUDA(ctx, cudaMemcpyAsync(buf[i]->p, host[i], bytes, cudaMemcpyHostToDevice, ctx->stream));
+  }
+  if ((st = spt_kv_read_device(ctx, cache, layer, &dev, kKvF32, k ? buf[0]->p : nullptr, 0, v ? buf[1]->p : nullptr,
+                               0)))
+    return st;
+  for (int i = 0; i < 2; ++i)
+    if (host[i]) SPT_CUDA(ctx, cudaMemcpyAsync(host[i], buf[i]->p, bytes, cudaMemcpyDeviceToHost, ctx->stream));
+  SPT_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  return SPT_OK;
+}
+
+spt_status spt_attention(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
+                         const spt_attention_config *cfg, const float *q, int64_t q_len, float *out,
+                         int64_t out_len, const volatile int32_t *cancel) {
+  spt_status st = kv_call(ctx, cache, layer, rows);
+  if (st) return st;
+  if ((st = attention_config(ctx, cache, cfg))) return st;
+  const int64_t n = rows->tokens * cfg->heads * cache->cfg.head_dim;
+  if (q_len != n || out_len != n)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "expected %lld query and output elements, got %lld and %lld", (long long)n,
+                (long long)q_len, (long long)out_len);
+  if (n > 0 && (!q || !out)) return fail(ctx, SPT_ERR_NULL_ARG, "nil query or output rows");
+  if (ranges_overlap(q, n * 4, out, n * 4))
+    return fail(ctx, SPT_ERR_OVERLAP, "query and output rows must not overlap");
+  if ((st = kv_host_rows(ctx, cache, rows))) return st;
+  if (canceled(cancel)) return fail(ctx, SPT_ERR_CANCELED, "context canceled");
+  if ((st = require_device(ctx))) return st;
+  if (n == 0) return SPT_OK;
+  spt_kv_rows dev;
+  if ((st = kv_stage_rows(ctx, cache, rows, &dev))) return st;
+  const size_t bytes = sizeof(float) * (size_t)n;
+  SPT_CUDA(ctx, cache->hin.ensure(bytes));
+  SPT_CUDA(ctx, cache->hout.ensure(bytes));
+  SPT_CUDA(ctx, cudaMemcpyAsync(cache->hin.p, q, bytes, cudaMemcpyHostToDevice, ctx->stream));
+  // rows of no sequence come back as they were
+  SPT_CUDA(ctx, cudaMemcpyAsync(cache->hout.p, out, bytes, cudaMemcpyHostToDevice, ctx->stream));
+  spt_attention_config dcfg = *cfg;
+  if (cfg->sinks) {
+    SPT_CUDA(ctx, cache->hsmall.ensure(sizeof(float) * (size_t)cfg->heads));
+    SPT_CUDA(ctx, cudaMemcpyAsync(cache->hsmall.p, cfg->sinks, sizeof(float) * (size_t)cfg->heads,
+                                  cudaMemcpyHostToDevice, ctx->stream));
+    dcfg.sinks = cache->hsmall.as<float>();
+  }
+  if ((st = spt_attention_device(ctx, cache, layer, &dev, &dcfg, kKvF32, cache->hin.p, 0, cache->hout.p, 0)))
+    return st;
+  SPT_CUDA(ctx, cudaMemcpyAsync(out, cache->hout.p, bytes, cudaMemcpyDeviceToHost, ctx->stream));
+  SPT_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  return SPT_OK;
+}
+
+spt_status spt_beam_validate(spt_context *ctx, const spt_beam_config *cfg) {
+  if (!ctx) return fail(nullptr, SPT_ERR_NULL_ARG, "nil context");
+  return beam_config(ctx, cfg);
+}
+
+spt_status spt_beam_create(spt_context *ctx, const spt_beam_config *cfg, spt_beam **out) {
+  if (!ctx || !out) return fail(ctx, SPT_ERR_NULL_ARG, "nil context or output");
+  *out = nullptr;
+  spt_status st = beam_config(ctx, cfg);
+  if (st) return st;
+  if ((st = require_device(ctx))) return st;
+  spt_beam *b = new (std::nothrow) spt_beam();
+  if (!b) return fail(ctx, SPT_ERR_CUDA, "beam search: out of host memory");
+  b->ctx = ctx;
+  b->cfg = *cfg;
+  const cudaError_t e =
+      b->work.ensure(beam_workspace_bytes(cfg->batch, cfg->beams, cfg->vocab, (int)cfg->keep, ctx->sm_count));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    spt_beam_destroy(b);
+    return cuda_fail(ctx, e, "beam search workspace");
+  }
+  *out = b;
+  return SPT_OK;
+}
+
+void spt_beam_destroy(spt_beam *b) {
+  if (!b) return;
+  if (b->ctx && b->ctx->has_device) {
+    cudaSetDevice(b->ctx->device);
+    cudaStreamSynchronize(b->ctx->stream);
+  }
+  for (DevBuf *d : {&b->work, &b->hlogits, &b->hsmall}) d->release();
+  delete b;
+}
+
+spt_status spt_beam_select_device(spt_context *ctx, spt_beam *b, int32_t type, const void *logits,
+                                  int64_t row_stride, const float *scores, const uint8_t *finished,
+                                  int64_t end_token, float *out_scores, int32_t *out_parents, int32_t *out_tokens) {
+  if (!ctx || !b || !logits || !scores || !out_scores || !out_parents || !out_tokens)
+    return fail(ctx, SPT_ERR_NULL_ARG, "nil beam search argument");
+  if (b->ctx != ctx) return fail(ctx, SPT_ERR_DIMENSIONS, "beam search belongs to another context");
+  spt_status st = row_array(ctx, logits, type, b->cfg.vocab, b->cfg.batch * b->cfg.beams, &row_stride);
+  if (st) return st;
+  if (!aligned(scores, 4) || !aligned(out_scores, 4) || !aligned(out_parents, 4) || !aligned(out_tokens, 4))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "beam search arrays not aligned to 4 bytes");
+  if (finished && (end_token < 0 || end_token >= b->cfg.vocab))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "end token %lld outside the vocabulary of %lld", (long long)end_token,
+                (long long)b->cfg.vocab);
+  if ((st = require_device(ctx))) return st;
+  BeamArgs a;
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.scores = scores;
+  a.finished = finished;
+  a.type = type;
+  a.batch = b->cfg.batch;
+  a.beams = b->cfg.beams;
+  a.vocab = b->cfg.vocab;
+  a.keep = (int)b->cfg.keep;
+  a.end_token = end_token;
+  a.out_scores = out_scores;
+  a.out_parents = out_parents;
+  a.out_tokens = out_tokens;
+  a.work = b->work.p;
+  a.sm_count = ctx->sm_count;
+  SPT_CUDA(ctx, launch_beam_select(a, ctx->stream));
+  ctx->kernels_last = 2;
+  return SPT_OK;
+}
+
+spt_status spt_beam_select(spt_context *ctx, spt_beam *b, const float *logits, int64_t logits_len,
+                           const float *scores, const uint8_t *finished, int64_t end_token, float *out_scores,
+                           int32_t *out_parents, int32_t *out_tokens) {
+  if (!ctx || !b || !logits || !scores || !out_scores || !out_parents || !out_tokens)
+    return fail(ctx, SPT_ERR_NULL_ARG, "nil beam search argument");
+  if (b->ctx != ctx) return fail(ctx, SPT_ERR_DIMENSIONS, "beam search belongs to another context");
+  const int64_t rows = b->cfg.batch * b->cfg.beams, n = rows * b->cfg.vocab, kept = b->cfg.batch * b->cfg.keep;
+  if (logits_len != n)
+    return fail(ctx, SPT_ERR_DIMENSIONS, "expected %lld logits, got %lld", (long long)n, (long long)logits_len);
+  if (finished && (end_token < 0 || end_token >= b->cfg.vocab))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "end token %lld outside the vocabulary of %lld", (long long)end_token,
+                (long long)b->cfg.vocab);
+  spt_status st = require_device(ctx);
+  if (st) return st;
+  cudaStream_t s = ctx->stream;
+  SPT_CUDA(ctx, b->hlogits.ensure(sizeof(float) * (size_t)n));
+  SPT_CUDA(ctx, b->hsmall.ensure((size_t)(kept * 12 + rows * 5)));
+  float *d_out = b->hsmall.as<float>(), *d_scores = d_out + 3 * kept;
+  int32_t *d_par = reinterpret_cast<int32_t *>(d_out + kept), *d_tok = d_par + kept;
+  uint8_t *d_fin = reinterpret_cast<uint8_t *>(d_scores + rows);
+  SPT_CUDA(ctx, cudaMemcpyAsync(b->hlogits.p, logits, sizeof(float) * (size_t)n, cudaMemcpyHostToDevice, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(d_scores, scores, sizeof(float) * (size_t)rows, cudaMemcpyHostToDevice, s));
+  if (finished) SPT_CUDA(ctx, cudaMemcpyAsync(d_fin, finished, (size_t)rows, cudaMemcpyHostToDevice, s));
+  if ((st = spt_beam_select_device(ctx, b, kKvF32, b->hlogits.p, 0, d_scores, finished ? d_fin : nullptr, end_token,
+                                   d_out, d_par, d_tok)))
+    return st;
+  SPT_CUDA(ctx, cudaMemcpyAsync(out_scores, d_out, sizeof(float) * (size_t)kept, cudaMemcpyDeviceToHost, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(out_parents, d_par, sizeof(int32_t) * (size_t)kept, cudaMemcpyDeviceToHost, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(out_tokens, d_tok, sizeof(int32_t) * (size_t)kept, cudaMemcpyDeviceToHost, s));
+  SPT_CUDA(ctx, cudaStreamSynchronize(s));
+  return SPT_OK;
+}
+
+spt_status spt_kv_reorder_device(spt_context *ctx, spt_kv_cache *cache, int64_t batch, int64_t beams,
+                                 int64_t max_pages, const int32_t *parents, int64_t parents_stride,
+                                 const int32_t *table, const int32_t *lengths, const int32_t *spare,
+                                 int32_t *table_out, int32_t *lengths_out, uint8_t *copied) {
+  spt_status st = reorder_args(ctx, cache, batch, beams, max_pages, parents, parents_stride, table, lengths, spare,
+                               table_out, lengths_out, copied);
+  if (st) return st;
+  if ((st = require_device(ctx))) return st;
+  KvReorder r;
+  r.parents = parents;
+  r.parents_stride = parents_stride;
+  r.table = table;
+  r.lengths = lengths;
+  r.spare = spare;
+  r.table_out = table_out;
+  r.lengths_out = lengths_out;
+  r.copied = copied;
+  r.batch = batch;
+  r.beams = beams;
+  r.max_pages = max_pages;
+  SPT_CUDA(ctx, launch_kv_reorder(cache->pool.as<uint8_t>(), cache->cfg.layers, cache->layer_bytes, kv_layer(cache, 0),
+                                  r, ctx->stream));
+  ctx->kernels_last = 1;
+  return SPT_OK;
+}
+
+spt_status spt_kv_reorder(spt_context *ctx, spt_kv_cache *cache, int64_t batch, int64_t beams, int64_t max_pages,
+                          const int32_t *parents, int64_t parents_stride, const int32_t *table,
+                          const int32_t *lengths, const int32_t *spare, int32_t *table_out, int32_t *lengths_out,
+                          uint8_t *copied) {
+  spt_status st = reorder_args(ctx, cache, batch, beams, max_pages, parents, parents_stride, table, lengths, spare,
+                               table_out, lengths_out, copied);
+  if (st) return st;
+  const int64_t n = batch * beams, page = cache->cfg.page_tokens;
+  for (int64_t s = 0; s < n; ++s) {
+    const int64_t len = lengths[s], used = len > 0 ? (len + page - 1) / page : 0;
+    if (len < 0 || used > max_pages)
+      return fail(ctx, SPT_ERR_DIMENSIONS, "sequence %lld: a length of %lld on %lld pages", (long long)s,
+                  (long long)len, (long long)max_pages);
+    for (int64_t i = 0; i < used; ++i)
+      if (table[s * max_pages + i] < 0 || table[s * max_pages + i] >= cache->cfg.pages)
+        return fail(ctx, SPT_ERR_DIMENSIONS, "sequence %lld: page %d outside the pool", (long long)s,
+                    table[s * max_pages + i]);
+    const int32_t p = parents[s / beams * parents_stride + s % beams];
+    if (p < -1 || p >= beams) return fail(ctx, SPT_ERR_DIMENSIONS, "parent %d of %lld beams", p, (long long)beams);
+    if (spare[s] < -1 || spare[s] >= cache->cfg.pages)
+      return fail(ctx, SPT_ERR_DIMENSIONS, "spare page %d outside the pool", spare[s]);
+    bool later = false;
+    for (int64_t i = s / beams * parents_stride; i < s / beams * parents_stride + s % beams; ++i)
+      later |= parents[i] == p;
+    if (p >= 0 && later && lengths[s / beams * beams + p] % page != 0 && spare[s] < 0)
+      return fail(ctx, SPT_ERR_DIMENSIONS, "sequence %lld needs a spare page", (long long)s);
+  }
+  if ((st = require_device(ctx))) return st;
+  cudaStream_t s = ctx->stream;
+  const int64_t n_par = (batch - 1) * parents_stride + beams, n_tab = n * max_pages;
+  SPT_CUDA(ctx, cache->hint.ensure(sizeof(int32_t) * (size_t)(n_par + 2 * n_tab + 3 * n) + (size_t)n));
+  int32_t *d_par = cache->hint.as<int32_t>(), *d_tab = d_par + n_par, *d_len = d_tab + n_tab, *d_spare = d_len + n,
+          *d_tab2 = d_spare + n, *d_len2 = d_tab2 + n_tab;
+  uint8_t *d_copied = reinterpret_cast<uint8_t *>(d_len2 + n);
+  SPT_CUDA(ctx, cudaMemcpyAsync(d_par, parents, sizeof(int32_t) * (size_t)n_par, cudaMemcpyHostToDevice, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(d_tab, table, sizeof(int32_t) * (size_t)n_tab, cudaMemcpyHostToDevice, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(d_len, lengths, sizeof(int32_t) * (size_t)n, cudaMemcpyHostToDevice, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(d_spare, spare, sizeof(int32_t) * (size_t)n, cudaMemcpyHostToDevice, s));
+  if ((st = spt_kv_reorder_device(ctx, cache, batch, beams, max_pages, d_par, parents_stride, d_tab, d_len, d_spare,
+                                  d_tab2, d_len2, d_copied)))
+    return st;
+  SPT_CUDA(ctx, cudaMemcpyAsync(table_out, d_tab2, sizeof(int32_t) * (size_t)n_tab, cudaMemcpyDeviceToHost, s));
+  SPT_CUDA(ctx, cudaMemcpyAsync(lengths_out, d_len2, sizeof(int32_t) * (size_t)n, cudaMemcpyDeviceToHost, s));
+  if (copied) SPT_CUDA(ctx, cudaMemcpyAsync(copied, d_copied, (size_t)n, cudaMemcpyDeviceToHost, s));
+  SPT_CUDA(ctx, cudaStreamSynchronize(s));
+  return SPT_OK;
 }
 
 }  // extern "C"
