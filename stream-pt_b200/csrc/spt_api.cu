@@ -663,7 +663,7 @@ spt_status forward_mma(spt_context *ctx, const LayerDev &L, const spt_moe_config
 
 // What gave up, from the code a bounded device wait recorded.
 const char *device_wait_name(int32_t code) {
-  return code >= 20 ? "expert-parallel peer exchange" : code == 9 ? "router" : "tensor-core GEMM";
+  return code >= 30 ? "attention over the KV cache" : code >= 20 ? "expert-parallel peer exchange" : code == 9 ? "router" : "tensor-core GEMM";
 }
 
 spt_status check_device_error(spt_context *ctx) {
@@ -3666,7 +3666,13 @@ spt_status spt_kv_cache_create(spt_context *ctx, const spt_kv_config *cfg, spt_k
   const size_t bytes = (size_t)layer_bytes * (size_t)cfg->layers;
   cudaError_t e = c->pool.ensure(bytes);
   if (e == cudaSuccess) e = cudaMemsetAsync(c->pool.p, 0, bytes, ctx->stream);
-  if (e == cudaSuccess) e = c->partial.ensure(attn_workspace_bytes(ctx->sm_count, (int)(cfg->head_dim / 32)));
+  const int nb = (int)(cfg->head_dim / 32);
+  if (e == cudaSuccess)
+    e = c->partial.ensure(std::max(attn_workspace_bytes(ctx->sm_count, nb), attn_mma_workspace_bytes(ctx->sm_count, nb)));
+  if (e == cudaSuccess && !ctx->dev_err.p) {
+    e = ctx->dev_err.ensure(sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMemsetAsync(ctx->dev_err.p, 0, sizeof(int32_t), ctx->stream);
+  }
   if (e == cudaSuccess) e = c->arrive.ensure(attn_counter_bytes(ctx->sm_count));
   if (e == cudaSuccess) e = cudaMemsetAsync(c->arrive.p, 0, c->arrive.bytes, ctx->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
@@ -3754,6 +3760,9 @@ spt_status spt_attention_device(spt_context *ctx, spt_kv_cache *cache, int64_t l
   a.type = type;
   a.partial = cache->partial.as<float>();
   a.arrive = cache->arrive.as<int32_t>();
+  a.err = ctx->dev_err.as<int32_t>();
+  a.wait_shift = ctx->opt_wait_shift;
+  a.fault_tile = ctx->opt_fault_stage;
   a.sm_count = ctx->sm_count;
   SPT_CUDA(ctx, launch_attention(a, ctx->stream));
   ctx->kernels_last = 1;
@@ -3853,7 +3862,7 @@ spt_status spt_attention(spt_context *ctx, spt_kv_cache *cache, int64_t layer, c
     return st;
   SPT_CUDA(ctx, cudaMemcpyAsync(out, cache->hout.p, bytes, cudaMemcpyDeviceToHost, ctx->stream));
   SPT_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-  return SPT_OK;
+  return check_device_error(ctx);
 }
 
 spt_status spt_beam_validate(spt_context *ctx, const spt_beam_config *cfg) {

@@ -7,13 +7,7 @@
 //
 // in one pass over the cache with a running maximum and sum.  A row without
 // keys gives 0.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "spt_device.cuh"
-#include "spt_internal.cuh"
-#include "spt_kv.cuh"
-#include "spt_ptx.cuh"
+#include "spt_attn.cuh"
 
 namespace spt {
 namespace {
@@ -23,8 +17,8 @@ constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnStages = 3;
 constexpr int kAttnCtasPerSm = 2;
 constexpr int kAttnMinTiles = 8;     // a CTA's smallest share of the keys: a tile for each warp
+constexpr int kAttnHead = 4;         // an item's beginning and end, in tiles' time
 constexpr int kAttnMaxRows = 16;
-constexpr float kLog2e = 1.4426950408889634f;
 
 // D (16 x 8, f32) += A (16 x 16, f16) * B (16 x 8, f16)
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -33,141 +27,19 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
-__device__ __forceinline__ __half2 half2_of(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return bits(__floats2half2_rn(lo, hi)); }
-
-// The eight codes of a word as four f16 pairs of n - 8, exactly: pair i holds
-// nibbles i and i + 4.  A nibble under the exponent of 1024 is 1024 + n (or,
-// four bits higher, 1024 + 16 n).
-__device__ __forceinline__ void decode_word(uint32_t w, uint32_t (&e)[4]) {
-  const __half2 low = half2_of(0x64086408u);                      // 1032
-  const __half2 sixteenth = half2_of(0x2c002c00u), off = half2_of(0xd480d480u);  // 1/16, -72
-  const uint32_t v = w >> 8;
-  e[0] = bits(__hsub2(half2_of((w & 0x000f000fu) | 0x64006400u), low));
-  e[1] = bits(__hfma2(half2_of((w & 0x00f000f0u) | 0x64006400u), sixteenth, off));
-  e[2] = bits(__hsub2(half2_of((v & 0x000f000fu) | 0x64006400u), low));
-  e[3] = bits(__hfma2(half2_of((v & 0x00f000f0u) | 0x64006400u), sixteenth, off));
-}
-
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-__device__ __forceinline__ void load_row8(const void *p, int64_t at, int type, float (&x)[8]) {
-  if (type == kKvF32) {
-    const float *q = static_cast<const float *>(p) + at;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = q[i];
-  } else if (type == kKvF16) {
-    const __half *q = static_cast<const __half *>(p) + at;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __half2float(q[i]);
-  } else {
-    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p) + at;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(q[i]);
-  }
-}
-
-__device__ __forceinline__ void store_row4(void *p, int64_t at, int type, const float (&x)[4]) {
-  if (type == kKvF32) {
-    float *o = static_cast<float *>(p) + at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = x[i];
-  } else if (type == kKvF16) {
-    __half *o = static_cast<__half *>(p) + at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __float2half_rn(x[i]);
-  } else {
-    __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p) + at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __float2bfloat16_rn(x[i]);
-  }
-}
-
-// A sequence's new rows, and the tiles of keys that a block of `ROWS`
-// consecutive (row, head of the group) pairs sees.
-struct SeqRows {
-  int64_t start, len, n;
-};
-__device__ __forceinline__ SeqRows seq_rows(const AttnArgs &a, int64_t b) {
-  SeqRows s;
-  s.len = a.r.lengths[b];
-  if (s.len < 0) s.len = 0;
-  if (!a.r.offsets) {
-    s.start = b;
-    s.n = b < a.r.tokens ? 1 : 0;
-  } else {
-    s.start = a.r.offsets[b];
-    const int64_t end = a.r.offsets[b + 1];
-    s.n = s.start < 0 || end > a.r.tokens || end < s.start ? 0 : end - s.start;
-  }
-  return s;
-}
-struct KeyTiles {
-  int64_t first, last;  // tiles [first, last)
-  __device__ __forceinline__ int64_t units() const { return last > first ? last - first : 1; }
-};
-template <int ROWS>
-__device__ __forceinline__ KeyTiles key_tiles(const AttnArgs &a, const SeqRows &s, int64_t rb) {
-  const int64_t i0 = rb * ROWS / a.group;
-  int64_t i1 = (rb * ROWS + ROWS - 1) / a.group;
-  if (i1 > s.n - 1) i1 = s.n - 1;
-  int64_t hi = s.len - s.n + i1 + 1;
-  const int64_t cap = a.r.max_pages * a.c.page_tokens;
-  if (hi > cap) hi = cap;
-  int64_t lo = a.window > 0 ? s.len - s.n + i0 - a.window + 1 : 0;
-  if (lo < 0) lo = 0;
-  KeyTiles t = {0, 0};
-  if (hi > lo) t.first = lo / kKvTile, t.last = (hi + kKvTile - 1) / kKvTile;
-  return t;
-}
-template <int ROWS>
-__device__ __forceinline__ int64_t row_blocks(const AttnArgs &a, const SeqRows &s) {
-  return (s.n * a.group + ROWS - 1) / ROWS;
-}
-// Units (tiles, at least one an item) of one key head of a sequence.
-template <int ROWS>
-__device__ int64_t head_units(const AttnArgs &a, const SeqRows &s) {
-  const int64_t blocks = row_blocks<ROWS>(a, s);
-  int64_t u = 0;
-  for (int64_t rb = 0; rb < blocks; ++rb) u += key_tiles<ROWS>(a, s, rb).units();
-  return u;
-}
-
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t *scratch) {
-#pragma unroll
-  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int64_t s = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) s += scratch[w];
-  __syncthreads();
-  return s;
-}
-
 // The work, B = NB blocks of 32 dims, TERMS f16 terms of q and of the softmax
 // weights (2 for f32 rows: 22 bits each; 1 for f16 and bf16 rows), NT blocks
 // of 8 rows.
 //
-// All (sequence, key head, row block) items in a row are cut into equal
-// shares of 16-key tiles, one share a CTA, so ragged batches load every SM
-// alike and a single long sequence is split over all of them.  Within a share
-// the warps take steps of up to KS tiles in turn, each warp with its own
-// cp.async ring and its own running maximum and sum; they meet in shared
-// memory at the item's end.  An item that several CTAs share is joined by the
-// one that arrives last, in the order of the shares, so the result does not
-// depend on the order of arrival.
+// Within its share of the 16-key tiles (AttnWalk) a CTA's warps take steps of
+// up to KS tiles in turn, each warp with its own cp.async ring and its own
+// running maximum and sum; they meet in shared memory at the item's end.
 //
 // Products.  S (rows x keys) = Q K^T with the rows' two f16 terms stacked
 // along M (TERMS 2) or two row blocks stacked (TERMS 1), codes n - 8 exact in
@@ -175,44 +47,32 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t *scratch) {
 // O^T (dims x rows) = V^T P^T with the values' scales applied to the weights
 // of each 32-dim block before their split into f16 terms.  S's fragment is
 // the layout that P^T's operand needs.
-template <int NB, int TERMS, int NT>
+template <int NB, typename IO, int NT>
 struct Attn {
+  static constexpr int kTerms = sizeof(IO) == 4 ? 2 : 1;
   static constexpr int kDim = NB * 32, kRows = NT * 8;
   static constexpr int kTile = kv_tile_bytes(NB);
   static constexpr int kSteps = NB <= 2 ? 4 : 2;  // tiles in a step at most
   static constexpr int kRing = kAttnStages * kSteps * kTile;
   static constexpr int kRedBytes = kAttnWarps * kRows * (kDim + 2) * 4;
   static constexpr int kSmem = kAttnWarps * kRing > kRedBytes ? kAttnWarps * kRing : kRedBytes;
-  static constexpr int kMinCtas = NB <= 2 && TERMS * NT < 4 ? 2 : 1;
-  static constexpr int kQ = TERMS == 2 ? NT : (NT + 1) / 2;  // A operands of 16 rows
+  static constexpr int kMinCtas = NB <= 2 && kTerms * NT < 4 ? 2 : 1;
+  static constexpr int kQ = kTerms == 2 ? NT : (NT + 1) / 2;  // A operands of 16 rows
 };
 
-// out row from its sums: acc and l stand for 2^ref times their value.
+template <typename IO>
 __device__ __forceinline__ void finish4(const AttnArgs &a, int64_t row, int head, int dim, float ref, float l,
                                         const float (&acc)[4], int head_dim) {
-  float o[4];
-  float up = 1.0f, below = l;
-  if (a.sinks) {
-    const float sink = a.sinks[head] * kLog2e;
-    const float top = fmaxf(ref, sink);
-    if (top > -INFINITY) {
-      up = exp2f(ref - top);
-      below = l * up + exp2f(sink - top);
-    }
-    if (isnan(sink)) below = sink;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = below == 0.0f ? 0.0f : acc[i] * up / below;
-  store_row4(a.out, row * a.out_stride + (int64_t)head * head_dim + dim, a.type, o);
+  const float f = row_factor(a, head, ref, l);
+  const float o[4] = {acc[0] * f, acc[1] * f, acc[2] * f, acc[3] * f};
+  store_row4(static_cast<IO *>(a.out) + row * a.out_stride + (int64_t)head * head_dim + dim, a.out_vec, o);
 }
 
-template <int NB, int TERMS, int NT>
-__global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k_attn(const AttnArgs a) {
-  using C = Attn<NB, TERMS, NT>;
-  constexpr int ROWS = C::kRows, DIM = C::kDim, KS = C::kSteps, TILE = C::kTile, W = kAttnWarps;
+template <int NB, typename IO, int NT>
+__global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_attn(const AttnArgs a) {
+  using C = Attn<NB, IO, NT>;
+  constexpr int TERMS = C::kTerms, ROWS = C::kRows, DIM = C::kDim, KS = C::kSteps, TILE = C::kTile, W = kAttnWarps;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t scratch[kAttnWarps];
-  __shared__ int64_t found[2];
   __shared__ int last_cta;
   __shared__ uint32_t okmask[kAttnWarps][kAttnStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -222,70 +82,12 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's share ------------------------------------------------------
-  const int heads = a.c.kv_heads;
-  int64_t total = 0;
-  for (int64_t b = tid; b < a.r.sequences; b += kAttnThreads) total += head_units<ROWS>(a, seq_rows(a, b)) * heads *
-                                                                        (seq_rows(a, b).n > 0);
-  total = block_sum(total, scratch);
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  if (share < kAttnMinTiles) share = kAttnMinTiles;
-  const int64_t begin = (int64_t)blockIdx.x * share;
-  const int64_t end = begin + share < total ? begin + share : total;
-  if (begin >= total) return;
-  {  // the sequence that holds unit `begin`, and the units before it
-    int64_t before = 0;
-    for (int64_t b0 = 0; b0 < a.r.sequences; b0 += kAttnThreads) {
-      const int64_t b = b0 + tid;
-      int64_t v = 0;
-      if (b < a.r.sequences) {
-        const SeqRows s = seq_rows(a, b);
-        if (s.n > 0) v = head_units<ROWS>(a, s) * heads;
-      }
-      int64_t up = v;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int64_t o = __shfl_up_sync(0xffffffffu, up, m);
-        if (lane >= m) up += o;
-      }
-      if (lane == 31) scratch[warp] = up;
-      __syncthreads();
-      int64_t all = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        if (w < warp) up += scratch[w];
-        all += scratch[w];
-      }
-      const int64_t first = before + up - v;
-      if (begin >= first && begin < first + v) found[0] = b, found[1] = first;
-      before += all;
-      __syncthreads();
-      if (before > begin) break;
-    }
-  }
-  int64_t b = found[0];
-  SeqRows seq = seq_rows(a, b);
-  int64_t unit = begin, rb = 0;
-  int head = 0;
-  int64_t item_begin = found[1];  // unit at which the current item starts
-  {
-    const int64_t per_head = head_units<ROWS>(a, seq);
-    head = (int)((begin - item_begin) / per_head);
-    item_begin += head * per_head;
-  }
-  KeyTiles tiles = key_tiles<ROWS>(a, seq, 0);
-  while (item_begin + tiles.units() <= begin) {
-    item_begin += tiles.units();
-    tiles = key_tiles<ROWS>(a, seq, ++rb);
-  }
-
-  while (true) {
-    // ---- one item: tiles [ta, tb) of it are this CTA's --------------------------
-    const int64_t units = tiles.units();
-    const int64_t skip = unit - item_begin;
-    const int64_t take = (units - skip < end - unit) ? units - skip : end - unit;
-    const int64_t ta = tiles.first + skip;
-    const int64_t tb = tiles.last > tiles.first ? ta + take : ta;
+  AttnWalk<ROWS, kKvTile, kAttnHead> w;
+  if (!w.template begin<kAttnThreads>(a, kAttnMinTiles)) return;
+  do {
+    const SeqRows &seq = w.seq;
+    const int64_t rb = w.rb, ta = w.first_tile(), tb = w.last_tile();  // tiles [ta, tb) of the item are this CTA's
+    const int head = w.head;
 
     // this lane's rows, one of each row block: position limits and q
     int64_t key_lo[NT], key_hi[NT];
@@ -301,10 +103,10 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
     int64_t all_lo = 0, all_hi = INT64_MAX;  // keys that every row of the warp sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int64_t r = rb * ROWS + nt * 8 + g, i = r / a.group;
+      const int64_t r = rb * ROWS + nt * 8 + g, i = (uint32_t)r / (uint32_t)a.group;
       const bool live = i < seq.n;
       const int qh = head * a.group + (int)(r - i * a.group);
-      key_hi[nt] = live ? seq.len - seq.n + i + 1 : 0;
+      key_hi[nt] = live ? (int64_t)seq.len - seq.n + i + 1 : 0;
       key_lo[nt] = a.window > 0 && live ? key_hi[nt] - a.window : 0;
       if (live) {
         all_lo = key_lo[nt] > all_lo ? key_lo[nt] : all_lo;
@@ -316,7 +118,8 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
       float x[NB][8], top = 0.0f;
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
-        if (live) load_row8(a.q, (seq.start + i) * a.q_stride + (int64_t)qh * DIM + k * 32 + t * 8, a.type, x[k]);
+        if (live)
+          load_row<IO, 8>(static_cast<const IO *>(a.q) + (seq.start + i) * a.q_stride + (int64_t)qh * DIM + k * 32 + t * 8, a.q_vec, x[k]);
         else
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
@@ -373,7 +176,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
     const int per_step = count >= (int64_t)KS * W ? KS : count <= W ? 1 : (int)((count + W - 1) / W);
     const int64_t steps = (count + per_step - 1) / per_step;
     const int tiles_per_page = a.c.page_tokens / kKvTile;
-    const int32_t *pages = a.r.table + b * a.r.max_pages;
+    const int32_t *pages = a.r.table + w.b * a.r.max_pages;
     auto page_of = [&](int64_t j) -> int32_t {  // lane i: page of tile i of this warp's step j
       const int64_t step = warp + j * W, tile = ta + step * per_step + lane;
       return step < steps && lane < per_step && tile < tb ? pages[tile / tiles_per_page] : -1;
@@ -618,10 +421,9 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
               make_float4(o[nt][k][0][x], o[nt][k][0][2 + x], o[nt][k][1][x], o[nt][k][1][2 + x]);
     }
     __syncthreads();
-    const bool whole = take == units;
-    const int64_t first_cta = item_begin / share, last_share = (item_begin + units - 1) / share;
-    // an item cut by shares: its first CTA keeps its part in slot 1, every other in slot 0
-    float *slot = a.partial + ((int64_t)blockIdx.x * 2 + (blockIdx.x == first_cta)) * (ROWS * (DIM + 2));
+    const bool whole = w.whole();
+    const int64_t first_cta = w.first_cta(), last_share = w.last_cta();
+    float *slot = part_slot<ROWS, DIM>(a, blockIdx.x, first_cta);
     for (int x = tid; x < ROWS * DIM / 4; x += kAttnThreads) {
       const int r = x / (DIM / 4), dim = x % (DIM / 4) * 4;
       float top = -INFINITY;
@@ -637,9 +439,9 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
         acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
       }
       if (whole) {
-        const int64_t rr = rb * ROWS + r, i = rr / a.group;
+        const int64_t rr = rb * ROWS + r, i = (uint32_t)rr / (uint32_t)a.group;
         if (i < seq.n)
-          finish4(a, seq.start + i, head * a.group + (int)(rr - i * a.group), dim, top, sum, acc, DIM);
+          finish4<IO>(a, seq.start + i, head * a.group + (int)(rr - i * a.group), dim, top, sum, acc, DIM);
       } else {
         *reinterpret_cast<float4 *>(slot + r * DIM + dim) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         if (dim == 0) slot[ROWS * DIM + r] = top, slot[ROWS * DIM + ROWS + r] = sum;
@@ -658,55 +460,46 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, TERMS, NT>::kMinCtas) k
         __threadfence();
         for (int x = tid; x < ROWS * DIM / 4; x += kAttnThreads) {
           const int r = x / (DIM / 4), dim = x % (DIM / 4) * 4;
-          const int64_t rr = rb * ROWS + r, i = rr / a.group;
+          const int64_t rr = rb * ROWS + r, i = (uint32_t)rr / (uint32_t)a.group;
           if (i >= seq.n) continue;
           float top = -INFINITY;
           for (int64_t c = first_cta; c <= last_share; ++c)
-            top = fmaxf(top, __ldcg(a.partial + (c * 2 + (c == first_cta)) * (ROWS * (DIM + 2)) + ROWS * DIM + r));
+            top = fmaxf(top, __ldcg(part_slot<ROWS, DIM>(a, c, first_cta) + ROWS * DIM + r));
           float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
           for (int64_t c = first_cta; c <= last_share; ++c) {
-            const float *p = a.partial + (c * 2 + (c == first_cta)) * (ROWS * (DIM + 2));
+            const float *p = part_slot<ROWS, DIM>(a, c, first_cta);
             const float rw = __ldcg(p + ROWS * DIM + r);
             const float f = rw == -INFINITY ? 0.0f : exp2f(rw - top);
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + r * DIM + dim));
             sum += __ldcg(p + ROWS * DIM + ROWS + r) * f;
             acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
           }
-          finish4(a, seq.start + i, head * a.group + (int)(rr - i * a.group), dim, top, sum, acc, DIM);
+          finish4<IO>(a, seq.start + i, head * a.group + (int)(rr - i * a.group), dim, top, sum, acc, DIM);
         }
       }
     }
     __syncthreads();
-
-    // ---- the next item --------------------------------------------------------------
-    unit += take;
-    if (unit >= end) break;
-    item_begin += units;
-    if (++rb >= row_blocks<ROWS>(a, seq)) {
-      rb = 0;
-      if (++head >= heads) {
-        head = 0;
-        do seq = seq_rows(a, ++b);
-        while (seq.n == 0);
-      }
-    }
-    tiles = key_tiles<ROWS>(a, seq, rb);
-  }
+  } while (w.next(a));
 }
 
-template <int NB, int TERMS, int NT>
+template <int NB, typename IO, int NT>
 cudaError_t launch(const AttnArgs &a, cudaStream_t stream) {
-  using C = Attn<NB, TERMS, NT>;
-  const cudaError_t e = opt_in_smem(k_attn<NB, TERMS, NT>, C::kSmem);
+  using C = Attn<NB, IO, NT>;
+  const cudaError_t e = opt_in_smem(k_attn<NB, IO, NT>, C::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k_attn<NB, TERMS, NT>, dim3(a.sm_count * C::kMinCtas), dim3(kAttnThreads), C::kSmem, stream, a);
+  return launch_pdl(k_attn<NB, IO, NT>, dim3(a.sm_count * C::kMinCtas), dim3(kAttnThreads), C::kSmem, stream, a);
 }
 
-template <int NB>
+template <typename IO>
 cudaError_t launch_dims(const AttnArgs &a, cudaStream_t stream) {
   const bool two = a.r.offsets || a.group > 8;
-  if (a.type == kKvF32) return two ? launch<NB, 2, 2>(a, stream) : launch<NB, 2, 1>(a, stream);
-  return two ? launch<NB, 1, 2>(a, stream) : launch<NB, 1, 1>(a, stream);
+  switch (a.c.nb) {
+    case 1: return two ? launch<1, IO, 2>(a, stream) : launch<1, IO, 1>(a, stream);
+    case 2: return two ? launch<2, IO, 2>(a, stream) : launch<2, IO, 1>(a, stream);
+    case 3: return two ? launch<3, IO, 2>(a, stream) : launch<3, IO, 1>(a, stream);
+    case 4: return two ? launch<4, IO, 2>(a, stream) : launch<4, IO, 1>(a, stream);
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -716,13 +509,18 @@ size_t attn_workspace_bytes(int sm_count, int nb) {
 }
 size_t attn_counter_bytes(int sm_count) { return (size_t)sm_count * kAttnCtasPerSm * sizeof(int32_t); }
 
-cudaError_t launch_attention(const AttnArgs &a, cudaStream_t stream) {
+cudaError_t launch_attention(const AttnArgs &args, cudaStream_t stream) {
+  AttnArgs a = args;
   if (a.r.tokens <= 0 || a.r.sequences <= 0) return cudaSuccess;
-  switch (a.c.nb) {
-    case 1: return launch_dims<1>(a, stream);
-    case 2: return launch_dims<2>(a, stream);
-    case 3: return launch_dims<3>(a, stream);
-    case 4: return launch_dims<4>(a, stream);
+  if (a.r.tokens > INT32_MAX / a.group) return cudaErrorInvalidValue;
+  const int size = a.type == kKvF32 ? 4 : 2;
+  a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * size)) & 15) == 0;
+  a.out_vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * size)) & 15) == 0;
+  if (a.r.offsets && a.r.tokens * a.group > 32 * a.r.sequences) return launch_attention_mma(a, stream);
+  switch (a.type) {
+    case kKvF32: return launch_dims<float>(a, stream);
+    case kKvF16: return launch_dims<__half>(a, stream);
+    case kKvBF16: return launch_dims<__nv_bfloat16>(a, stream);
   }
   return cudaErrorInvalidValue;
 }

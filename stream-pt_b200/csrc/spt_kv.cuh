@@ -115,11 +115,18 @@ struct AttnArgs {
   int64_t window = 0;            // keys a row sees at most; 0: all
   int heads = 0, group = 0;
   int type = kKvF32;
+  bool q_vec = false, out_vec = false;  // rows start on 16 bytes
   float *partial = nullptr;      // attn_workspace_bytes()
   int32_t *arrive = nullptr;     // attn_counters() zeros between launches
+  int32_t *err = nullptr;        // set when a bounded wait gives up
+  int wait_shift = 31;
+  int fault_tile = -1;           // a test's: CTA 0 leaves out this tile's copies
   int sm_count = 148;
 };
 cudaError_t launch_attention(const AttnArgs &a, cudaStream_t stream);
+// The kernel for many rows of a key head (spt_attn_mma.cu), which launch_attention picks.
+cudaError_t launch_attention_mma(const AttnArgs &a, cudaStream_t stream);
+size_t attn_mma_workspace_bytes(int sm_count, int nb);
 size_t attn_workspace_bytes(int sm_count, int nb);
 size_t attn_counter_bytes(int sm_count);
 

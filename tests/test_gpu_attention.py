@@ -183,6 +183,82 @@ def test_masked_places_hold_anything(ctx):
     cache.close()
 
 
+@pytest.mark.parametrize("type", list(TYPES))
+def test_masked_places_of_chunks_hold_anything(ctx, type):
+    """The same for chunks of rows: NaNs behind a row's position or before its window stay out
+    of it, and one in sight of some rows reaches those alone, in the value blocks that hold it."""
+    import torch
+    lengths, counts = [300, 200], [90, 40]
+    cache, table, held = filled(ctx, 15, lengths, 2, 64, 16)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(130, 16, 64, generator=gen, device="cuda").to(torch_type(type))
+    want = check(ctx, cache, table, held, lengths, counts, 16, type, window=50, q=q)
+    # positions 0 .. 150 of sequence 0 (its rows see 161 ..) and 0 .. 99 of sequence 1 (111 ..)
+    junk = torch.full((251, 2, 64), float("nan"), device="cuda")
+    dev = Device(table, [151, 100], [151, 100])
+    torch.cuda.synchronize()
+    cache.append_device(dev.batch, junk.data_ptr(), junk.data_ptr())
+    ctx.sync()
+    out = torch.zeros_like(q)
+    dev = Device(table, lengths, counts)
+    torch.cuda.synchronize()
+
+    def attend():
+        cache.attention_device(dev.batch, q.data_ptr(), out.data_ptr(), 16, TYPES[type], scale=0.125, window=50)
+        ctx.sync()
+
+    attend()
+    assert bool((out == want).all())
+    # a value block with a NaN at position 250 of sequence 0: head 1, dims 32 .. 63
+    k, v = (x.float()[250:251].contiguous() for x in held[0])
+    v = v.clone()
+    v[0, 1, 40] = float("nan")
+    one = Device(table[:1], [251], [1])
+    torch.cuda.synchronize()
+    cache.append_device(one.batch, k.data_ptr(), v.data_ptr())
+    ctx.sync()
+    attend()
+    hit = torch.zeros(130, 16, 64, dtype=torch.bool, device="cuda")
+    first = 250 - 210  # row of position 250; windows of 50 see it from there to position 299
+    hit[first:90, 8:, 32:] = True
+    assert bool(torch.isnan(out[hit]).all()) and bool((out[~hit] == want[~hit]).all())
+    # a key with one: every value of the rows that see it
+    k[0, 0, 3] = float("nan")
+    torch.cuda.synchronize()
+    cache.append_device(one.batch, k.data_ptr(), k.data_ptr())
+    ctx.sync()
+    attend()
+    assert bool(torch.isnan(out[first:90, :8]).all()) and bool((out[:first] == want[:first]).all())
+    assert bool((out[90:] == want[90:]).all())
+    cache.close()
+
+
+def test_waits_that_run_out(ctx):
+    """A tile that is never loaded: the waits for it give up, the call is reported as timed out, and
+    the next is right again."""
+    import torch
+    lengths, counts = [3000, 500], [300, 64]
+    cache, table, held = filled(ctx, 16, lengths, 2, 64, 16)
+    q = torch.randn(364, 16, 64, device="cuda")
+    out = torch.zeros_like(q)
+    dev = Device(table, lengths, counts)
+    torch.cuda.synchronize()
+    old = ctx.get_option(spt.OPT_WAIT_LIMIT)
+    ctx.set_option(spt.OPT_WAIT_LIMIT, 18)
+    ctx.set_option(spt.OPT_FAULT_STAGE, 2)
+    try:
+        cache.attention_device(dev.batch, q.data_ptr(), out.data_ptr(), 16, scale=0.125)
+        with pytest.raises(spt.SptError) as e:
+            ctx.sync()
+        assert e.value.status == spt.ERR_TIMEOUT
+    finally:
+        ctx.set_option(spt.OPT_WAIT_LIMIT, old)
+        ctx.set_option(spt.OPT_FAULT_STAGE, -1)
+    for _ in range(2):
+        check(ctx, cache, table, held, lengths, counts, 16, q=q)
+    cache.close()
+
+
 def test_bad_query_rows_stay_alone(ctx):
     """A NaN or an infinity in one row of q gives NaNs there and touches no other row."""
     import torch
