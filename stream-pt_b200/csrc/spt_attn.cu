@@ -16,9 +16,8 @@ constexpr int kAttnWarps = 8;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnStages = 3;
 constexpr int kAttnCtasPerSm = 2;
-constexpr int kAttnMinTiles = 8;     // a CTA's smallest share of the keys: a tile for each warp
+constexpr int kAttnMinTiles = 12;    // a CTA's smallest share: a tile for each warp
 constexpr int kAttnHead = 4;         // an item's beginning and end, in tiles' time
-constexpr int kAttnMaxRows = 16;
 
 // D (16 x 8, f32) += A (16 x 16, f16) * B (16 x 8, f16)
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -27,19 +26,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
 // The work, B = NB blocks of 32 dims, TERMS f16 terms of q and of the softmax
 // weights (2 for f32 rows: 22 bits each; 1 for f16 and bf16 rows), NT blocks
 // of 8 rows.
 //
 // Within its share of the 16-key tiles (AttnWalk) a CTA's warps take steps of
-// up to KS tiles in turn, each warp with its own cp.async ring and its own
-// running maximum and sum; they meet in shared memory at the item's end.
+// up to KS tiles in turn, each warp with its own ring of bulk copies and its own
+// running maximum and sum; they meet in shared memory at the item's end.  (With
+// a share a warp and no meeting, a long sequence left hundreds of parts to be
+// joined: one of 131,000 tokens took 212 us instead of 62.)
 //
 // Products.  S (rows x keys) = Q K^T with the rows' two f16 terms stacked
 // along M (TERMS 2) or two row blocks stacked (TERMS 1), codes n - 8 exact in
@@ -56,6 +51,8 @@ struct Attn {
   static constexpr int kRing = kAttnStages * kSteps * kTile;
   static constexpr int kRedBytes = kAttnWarps * kRows * (kDim + 2) * 4;
   static constexpr int kSmem = kAttnWarps * kRing > kRedBytes ? kAttnWarps * kRing : kRedBytes;
+  static constexpr int kSub = 2;                  // tiles of a step whose weights are taken at once
+  // CTAs on an SM: 16 warps of 128 registers, where that holds the fragments
   static constexpr int kMinCtas = NB <= 2 && kTerms * NT < 4 ? 2 : 1;
   static constexpr int kQ = kTerms == 2 ? NT : (NT + 1) / 2;  // A operands of 16 rows
 };
@@ -74,7 +71,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
   constexpr int TERMS = C::kTerms, ROWS = C::kRows, DIM = C::kDim, KS = C::kSteps, TILE = C::kTile, W = kAttnWarps;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last_cta;
-  __shared__ uint32_t okmask[kAttnWarps][kAttnStages];
+  __shared__ uint64_t bars[kAttnWarps][kAttnStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t *ring = smem + warp * C::kRing;
   float *red = reinterpret_cast<float *>(smem);  // [W][ROWS][DIM], then ref [W][ROWS], l [W][ROWS]
@@ -83,14 +80,20 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
   pdl_trigger();
 
   AttnWalk<ROWS, kKvTile, kAttnHead> w;
-  if (!w.template begin<kAttnThreads>(a, kAttnMinTiles)) return;
+  if (tid < W * kAttnStages) mbar_init(&bars[tid / kAttnStages][tid % kAttnStages], 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
+  if (!w.template begin<kAttnThreads>(a, kAttnMinTiles, blockIdx.x, gridDim.x)) return;
+  const uint32_t tiles_per_page = (uint32_t)a.c.page_tokens / kKvTile;
+  int stage = 0;  // of this warp's ring: the step to be read next
+  uint32_t phase = 0;
   do {
     const SeqRows &seq = w.seq;
-    const int64_t rb = w.rb, ta = w.first_tile(), tb = w.last_tile();  // tiles [ta, tb) of the item are this CTA's
+    const int rb = w.rb, ta = w.first_tile(), tb = w.last_tile();  // tiles [ta, tb) of the item are this CTA's
     const int head = w.head;
 
     // this lane's rows, one of each row block: position limits and q
-    int64_t key_lo[NT], key_hi[NT];
+    int key_lo[NT], key_hi[NT];
     float ref[NT], l[NT], cs[NT];
     bool fresh[NT];
     uint32_t qa[C::kQ][NB * 2][4];
@@ -100,14 +103,14 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
       for (int k = 0; k < NB * 2; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) qa[i][k][j] = 0;
-    int64_t all_lo = 0, all_hi = INT64_MAX;  // keys that every row of the warp sees
+    int all_lo = 0, all_hi = INT32_MAX;  // keys that every row of the warp sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int64_t r = rb * ROWS + nt * 8 + g, i = (uint32_t)r / (uint32_t)a.group;
+      const int r = rb * ROWS + nt * 8 + g, i = (int)((uint32_t)r / (uint32_t)a.group);
       const bool live = i < seq.n;
-      const int qh = head * a.group + (int)(r - i * a.group);
-      key_hi[nt] = live ? (int64_t)seq.len - seq.n + i + 1 : 0;
-      key_lo[nt] = a.window > 0 && live ? key_hi[nt] - a.window : 0;
+      const int qh = head * a.group + r - i * a.group;
+      key_hi[nt] = live ? seq.len - seq.n + i + 1 : 0;
+      key_lo[nt] = a.window > 0 && key_hi[nt] > a.window ? key_hi[nt] - (int)a.window : 0;
       if (live) {
         all_lo = key_lo[nt] > all_lo ? key_lo[nt] : all_lo;
         all_hi = key_hi[nt] < all_hi ? key_hi[nt] : all_hi;
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         if (live)
-          load_row<IO, 8>(static_cast<const IO *>(a.q) + (seq.start + i) * a.q_stride + (int64_t)qh * DIM + k * 32 + t * 8, a.q_vec, x[k]);
+          load_row<IO, 8>(static_cast<const IO *>(a.q) + (int64_t)(seq.start + i) * a.q_stride + (int64_t)qh * DIM + k * 32 + t * 8, a.q_vec, x[k]);
         else
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
     }
 #pragma unroll
     for (int m = 4; m < 32; m <<= 1) {
-      const int64_t lo = __shfl_xor_sync(0xffffffffu, all_lo, m), hi = __shfl_xor_sync(0xffffffffu, all_hi, m);
+      const int lo = __shfl_xor_sync(0xffffffffu, all_lo, m), hi = __shfl_xor_sync(0xffffffffu, all_hi, m);
       all_lo = lo > all_lo ? lo : all_lo;
       all_hi = hi < all_hi ? hi : all_hi;
     }
@@ -172,111 +175,108 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
     int vexp = -24;
 
     // ---- steps ------------------------------------------------------------------
-    const int64_t count = tb - ta;
-    const int per_step = count >= (int64_t)KS * W ? KS : count <= W ? 1 : (int)((count + W - 1) / W);
-    const int64_t steps = (count + per_step - 1) / per_step;
-    const int tiles_per_page = a.c.page_tokens / kKvTile;
-    const int32_t *pages = a.r.table + w.b * a.r.max_pages;
-    auto page_of = [&](int64_t j) -> int32_t {  // lane i: page of tile i of this warp's step j
-      const int64_t step = warp + j * W, tile = ta + step * per_step + lane;
-      return step < steps && lane < per_step && tile < tb ? pages[tile / tiles_per_page] : -1;
+    // step j of this warp: tiles ta + (warp + j W) per_step on.  Lane i of it looks
+    // after tile i: its page, read a step ahead, and its copy; tiles that follow
+    // one another in a page are copied at once.
+    const int count = tb - ta;
+    const int per_step = count >= KS * W ? KS : count <= W ? 1 : (count + W - 1) / W;
+    const int32_t *pages = a.r.table + (int64_t)w.b * a.r.max_pages;
+    int32_t page = -1;
+    uint32_t place = 0;
+    int asked = ta + warp * per_step, read = asked;  // first tiles of the step asked for next, read next
+    auto ask = [&](int tile0) {
+      const uint32_t tile = (uint32_t)(tile0 + lane), p = tile / tiles_per_page;
+      place = tile - p * tiles_per_page;
+      page = lane < per_step && (int)tile < tb ? __ldcg(pages + p) : -1;
     };
-    auto issue = [&](int64_t j, int32_t page) {
-      const int64_t step = warp + j * W, tile0 = ta + step * per_step;
-      const int stage = (int)(j % kAttnStages);
-      const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0 && page < a.c.pages);
-      if (lane == 0) okmask[warp][stage] = ok;
-      if (step < steps) {
-        for (int i = 0; i < per_step && tile0 + i < tb; ++i) {
-          const int32_t p = __shfl_sync(0xffffffffu, page, i);
-          if (!(ok >> i & 1)) continue;
-          const uint8_t *src = a.c.base + kv_tile_offset(a.c, p, head, (int)((tile0 + i) % tiles_per_page) * kKvTile);
-          uint8_t *dst = ring + (stage * KS + i) * TILE;
-#pragma unroll
-          for (int c = 0; c < (TILE / 16 + 31) / 32; ++c)
-            if (c * 32 + lane < TILE / 16) cp_async16(dst + (c * 32 + lane) * 16, src + (c * 32 + lane) * 16);
-        }
-      }
-      cp_async_commit();
-    };
-    int32_t page_next = page_of(0);
-#pragma unroll
-    for (int j = 0; j < kAttnStages - 1; ++j) {
-      issue(j, page_next);
-      page_next = page_of(j + 1);
-    }
-    for (int64_t j = 0; warp + j * W < steps; ++j) {
-      cp_async_wait<kAttnStages - 2>();
+    auto fetch = [&](int to) {  // the step that was asked for, into ring slot `to`
+      const bool good = page >= 0 && page < a.c.pages;
+      const uint32_t ok = __ballot_sync(0xffffffffu, good);
+      const uint32_t starts = __ballot_sync(0xffffffffu, good && (place == 0 || lane == 0 || !(ok >> (lane - 1) & 1)));
+      if (lane == 0) mbar_expect_tx(&bars[warp][to], __popc(ok) * TILE);
       __syncwarp();
-      issue(j + kAttnStages - 1, page_next);
-      page_next = page_of(j + kAttnStages);
-      const int stage = (int)(j % kAttnStages);
-      const int64_t tile0 = ta + (warp + j * W) * per_step;
-      const int64_t key0 = tile0 * kKvTile;
-      const uint32_t ok = okmask[warp][stage];
-      const uint8_t *buf = ring + stage * KS * TILE;
-      const int n_tiles = (int)(tb - tile0 < per_step ? tb - tile0 : per_step);
-      const bool edge = key0 < all_lo || key0 + n_tiles * kKvTile > all_hi || ok != (1u << n_tiles) - 1u;
-
+      if (starts >> lane & 1) {  // up to the next start or bad page
+        const uint32_t ends = (starts | ~ok) >> lane >> 1;
+        bulk_load(ring + (to * KS + lane) * TILE, a.c.base + kv_tile_offset(a.c, page, head, (int)place * kKvTile),
+                  (uint32_t)__ffs(ends) * TILE, &bars[warp][to]);
+      }
+      return ok;
+    };
+    uint32_t ok_now = 0, ok_next = 0;  // good pages of the steps under way
+    int slot = stage;
+    if (asked < tb) {
+      ask(asked);
+      ok_now = fetch(slot);
+      asked += W * per_step;
+      ask(asked);
+      if (++slot == kAttnStages) slot = 0;
+      if (asked < tb) ok_next = fetch(slot);
+      asked += W * per_step;
+      ask(asked);
+      if (++slot == kAttnStages) slot = 0;
+    }
+    // KU tiles, all of whose keys every row sees, or any
+    constexpr int KU = C::kSub;
+    auto step = [&](auto full_step, const uint8_t *buf, int key0, int n_tiles, uint32_t ok) {
+      constexpr bool FULL = decltype(full_step)::value;
       // S = Q K^T of the step, and the largest value scale of it
-      float s[KS][NT][4];
+      float2 s[KU][NT][2];  // of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
       uint32_t vmax = 0;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
+      for (int i = 0; i < KU; ++i) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) s[i][nt][x] = 0.0f;
-        if (i >= n_tiles || !(ok >> i & 1)) continue;
+        for (int nt = 0; nt < NT; ++nt) s[i][nt][0] = s[i][nt][1] = make_float2(0.0f, 0.0f);
+        if (!FULL && (i >= n_tiles || !(ok >> i & 1))) continue;
         const uint8_t *tile = buf + i * TILE;
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
           const uint2 kd = *reinterpret_cast<const uint2 *>(tile + kv_key_scales(NB) + t * NB * 8 + k * 8);
           const uint2 vd = *reinterpret_cast<const uint2 *>(tile + kv_value_scales(NB) + t * NB * 8 + k * 8);
           vmax = bits(__hmax2(half2_of(vmax), __hmax2(half2_of(vd.x & 0x7fff7fffu), half2_of(vd.y & 0x7fff7fffu))));
-          const uint2 w = *reinterpret_cast<const uint2 *>(tile + kv_word(NB, k, lane, 0));
-          const float2 d[2] = {__half22float2(half2_of(kd.x)), __half22float2(half2_of(kd.y))};
+          const uint2 word = *reinterpret_cast<const uint2 *>(tile + kv_word(NB, k, lane, 0));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const float2 d = __half22float2(half2_of(h ? kd.y : kd.x));
             uint32_t e[4];
-            decode_word(h ? w.y : w.x, e);
+            decode_word(h ? word.y : word.x, e);
 #pragma unroll
             for (int q = 0; q < C::kQ; ++q) {
               float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
               mma16816(c, qa[q][k * 2], e[0], e[1]);
               mma16816(c, qa[q][k * 2 + 1], e[2], e[3]);
+              const float2 c0 = make_float2(c[0], c[1]), c1 = make_float2(c[2], c[3]);
               if constexpr (TERMS == 2) {
-                s[i][q][2 * h] = fmaf(c[0] + c[2], d[h].x, s[i][q][2 * h]);
-                s[i][q][2 * h + 1] = fmaf(c[1] + c[3], d[h].y, s[i][q][2 * h + 1]);
+                s[i][q][h] = __ffma2_rn(__fadd2_rn(c0, c1), d, s[i][q][h]);
               } else {
-                s[i][2 * q][2 * h] = fmaf(c[0], d[h].x, s[i][2 * q][2 * h]);
-                s[i][2 * q][2 * h + 1] = fmaf(c[1], d[h].y, s[i][2 * q][2 * h + 1]);
-                if constexpr (NT > 1) {
-                  s[i][2 * q + 1][2 * h] = fmaf(c[2], d[h].x, s[i][2 * q + 1][2 * h]);
-                  s[i][2 * q + 1][2 * h + 1] = fmaf(c[3], d[h].y, s[i][2 * q + 1][2 * h + 1]);
-                }
+                s[i][2 * q][h] = __ffma2_rn(c0, d, s[i][2 * q][h]);
+                if constexpr (NT > 1) s[i][2 * q + 1][h] = __ffma2_rn(c1, d, s[i][2 * q + 1][h]);
               }
             }
           }
         }
       }
-      // weights: x = log2 of the weight
+      // a key of this lane: pair h of tile i, its x-th
+      auto hidden = [&](int nt, int i, int h, int x) {
+        const int key = key0 + i * kKvTile + 2 * t + 8 * h + x;
+        return key < key_lo[nt] || key >= key_hi[nt] || i >= n_tiles || !(ok >> i & 1);
+      };
+      // s becomes log2 of the weight
       bool high = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const float2 scale = make_float2(cs[nt], cs[nt]), off = make_float2(-ref[nt], -ref[nt]);
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < KU; ++i)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float v = fmaf(s[i][nt][x], cs[nt], -ref[nt]);
-            if (i >= n_tiles) v = -INFINITY;
-            if (edge) {
-              const int64_t key = key0 + i * kKvTile + 2 * t + (x & 1) + (x >> 1) * 8;
-              if (key < key_lo[nt] || key >= key_hi[nt] || !(ok >> i & 1)) v = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            float2 v = __ffma2_rn(s[i][nt][h], scale, off);
+            if (!FULL) {
+              if (hidden(nt, i, h, 0)) v.x = -INFINITY;
+              if (hidden(nt, i, h, 1)) v.y = -INFINITY;
             }
-            s[i][nt][x] = v;
-            top = fmaxf(top, v);
+            s[i][nt][h] = v;
+            top = fmaxf(top, fmaxf(v.x, v.y));
           }
         high |= top > (fresh[nt] ? -INFINITY : (float)(15 - vexp));
       }
@@ -294,9 +294,9 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
         for (int nt = 0; nt < NT; ++nt) {
           float top = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < KS; ++i)
+          for (int i = 0; i < KU; ++i)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) top = fmaxf(top, s[i][nt][x]);
+            for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(s[i][nt][h].x, s[i][nt][h].y));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           float most = top + ref[nt];
@@ -304,10 +304,11 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
           const bool none = most == -INFINITY;
           const float now = none ? 0.0f : most + (float)(ve - 7);
           const float factor = fresh[nt] ? 1.0f : exp2f(ref[nt] - now);
+          const float2 move = make_float2(ref[nt] - now, ref[nt] - now);
 #pragma unroll
-          for (int i = 0; i < KS; ++i)
+          for (int i = 0; i < KU; ++i)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[i][nt][x] += ref[nt] - now;
+            for (int h = 0; h < 2; ++h) s[i][nt][h] = __fadd2_rn(s[i][nt][h], move);
           l[nt] *= factor;
           ref[nt] = now;
           fresh[nt] = none;
@@ -323,14 +324,17 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
         vexp = ve;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < KU; ++i)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[i][nt][x] = exp2_fast(s[i][nt][x]);
-            l[nt] += s[i][nt][x];
+          for (int h = 0; h < 2; ++h) {
+            s[i][nt][h] = make_float2(exp2_fast(s[i][nt][h].x), exp2_fast(s[i][nt][h].y));
+            sum = __fadd2_rn(sum, s[i][nt][h]);
           }
+        l[nt] += sum.x + sum.y;
+      }
       // O^T += V^T P^T.  With two terms the step's products are summed from
       // zero and added in f32: the tensor cores' own additions lose bits of a
       // long sum.
@@ -346,45 +350,43 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
               for (int x = 0; x < 4; ++x) oc[nt][k][m][x] = 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        if (i >= n_tiles || !(ok >> i & 1)) continue;
+      for (int i = 0; i < KU; ++i) {
+        if (!FULL && (i >= n_tiles || !(ok >> i & 1))) continue;
         const uint8_t *tile = buf + i * TILE;
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
           const uint2 vd = *reinterpret_cast<const uint2 *>(tile + kv_value_scales(NB) + t * NB * 8 + k * 8);
-          const uint2 w = *reinterpret_cast<const uint2 *>(tile + kv_value_codes(NB) + kv_word(NB, k, lane, 0));
+          const uint2 word = *reinterpret_cast<const uint2 *>(tile + kv_value_codes(NB) + kv_word(NB, k, lane, 0));
           uint32_t e0[4], e1[4];
-          decode_word(w.x, e0);
-          decode_word(w.y, e1);
+          decode_word(word.x, e0);
+          decode_word(word.y, e1);
           const uint32_t a0[4] = {e0[0], e0[1], e1[0], e1[1]}, a1[4] = {e0[2], e0[3], e1[2], e1[3]};
-          const float2 d0 = __half22float2(half2_of(vd.x)), d1 = __half22float2(half2_of(vd.y));
-          const float d[4] = {d0.x, d0.y, d1.x, d1.y};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float p[4];
+            uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              p[x] = s[i][nt][x] * d[x];
-              if (edge) {  // a masked key's scale may be anything
-                const int64_t key = key0 + i * kKvTile + 2 * t + (x & 1) + (x >> 1) * 8;
-                if (key < key_lo[nt] || key >= key_hi[nt]) p[x] = 0.0f;
+            for (int h = 0; h < 2; ++h) {
+              float2 p = __fmul2_rn(s[i][nt][h], __half22float2(half2_of(h ? vd.y : vd.x)));
+              if (!FULL) {  // a masked key's scale may be anything
+                if (hidden(nt, i, h, 0)) p.x = 0.0f;
+                if (hidden(nt, i, h, 1)) p.y = 0.0f;
+              }
+              const __half2 r = __floats2half2_rn(p.x, p.y);
+              hi[h] = bits(r);
+              if constexpr (TERMS == 2) {
+                const float2 rest = __ffma2_rn(__half22float2(r), make_float2(-1.0f, -1.0f), p);
+                lo[h] = pack_half2(rest.x, rest.y);
               }
             }
             if constexpr (TERMS == 2) {
-              float hi[4];
-#pragma unroll
-              for (int x = 0; x < 4; ++x) hi[x] = __uint_as_float(__float_as_uint(p[x]) & 0xffffe000u);
-              const uint32_t b0 = pack_half2(hi[0], hi[1]), b1 = pack_half2(hi[2], hi[3]);
-              const uint32_t c0 = pack_half2(p[0] - hi[0], p[1] - hi[1]), c1 = pack_half2(p[2] - hi[2], p[3] - hi[3]);
-              mma16816(oc[nt][k][0], a0, b0, b1);
-              mma16816(oc[nt][k][1], a1, b0, b1);
-              mma16816(oc[nt][k][0], a0, c0, c1);
-              mma16816(oc[nt][k][1], a1, c0, c1);
+              mma16816(oc[nt][k][0], a0, lo[0], lo[1]);
+              mma16816(oc[nt][k][1], a1, lo[0], lo[1]);
+              mma16816(oc[nt][k][0], a0, hi[0], hi[1]);
+              mma16816(oc[nt][k][1], a1, hi[0], hi[1]);
             } else {
               // one term: 2^-11 of each weight at most, no more than the rounding of f16 and bf16 rows
-              const uint32_t b0 = pack_half2(p[0], p[1]), b1 = pack_half2(p[2], p[3]);
-              mma16816(o[nt][k][0], a0, b0, b1);
-              mma16816(o[nt][k][1], a1, b0, b1);
+              mma16816(o[nt][k][0], a0, hi[0], hi[1]);
+              mma16816(o[nt][k][1], a1, hi[0], hi[1]);
             }
           }
         }
@@ -397,10 +399,36 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) o[nt][k][m][x] += oc[nt][k][m][x];
+              for (int x = 0; x < 4; x += 2) {
+                const float2 v = __fadd2_rn(make_float2(o[nt][k][m][x], o[nt][k][m][x + 1]),
+                                            make_float2(oc[nt][k][m][x], oc[nt][k][m][x + 1]));
+                o[nt][k][m][x] = v.x, o[nt][k][m][x + 1] = v.y;
+              }
       }
+    };
+#pragma unroll 1
+    for (; read < tb; read += W * per_step) {
+      brief_wait(&bars[warp][stage], phase, a, 46);  // (this warp's own copies; a wait that gives up is reported)
+      __syncwarp();  // the slot read last is free: the step after the next goes there
+      uint32_t ok_then = 0;
+      if (asked < tb) ok_then = fetch(slot);
+      asked += W * per_step;
+      ask(asked);
+      if (++slot == kAttnStages) slot = 0;
+      int key0 = read * kKvTile, n_tiles = tb - read < per_step ? tb - read : per_step;
+      const uint8_t *buf = ring + stage * KS * TILE;
+      uint32_t ok = ok_now;
+#pragma unroll 1
+      for (; n_tiles > 0; n_tiles -= KU, key0 += KU * kKvTile, buf += KU * TILE, ok >>= KU) {
+        constexpr uint32_t all = (1u << KU) - 1u;
+        if (n_tiles >= KU && (ok & all) == all && key0 >= all_lo && key0 + KU * kKvTile <= all_hi)
+          step(std::true_type{}, buf, key0, KU, all);
+        else
+          step(std::false_type{}, buf, key0, n_tiles, ok);
+      }
+      ok_now = ok_next, ok_next = ok_then;
+      if (++stage == kAttnStages) stage = 0, phase ^= 1u;
     }
-    cp_async_wait<0>();
     __syncthreads();
 
     // ---- the warps' sums meet ----------------------------------------------------
@@ -422,62 +450,62 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
     }
     __syncthreads();
     const bool whole = w.whole();
-    const int64_t first_cta = w.first_cta(), last_share = w.last_cta();
-    float *slot = part_slot<ROWS, DIM>(a, blockIdx.x, first_cta);
+    const int first = w.first_share(), last = w.last_share();
+    float *part = part_slot<ROWS, DIM>(a, blockIdx.x, first);
     for (int x = tid; x < ROWS * DIM / 4; x += kAttnThreads) {
       const int r = x / (DIM / 4), dim = x % (DIM / 4) * 4;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, red_ref[w * ROWS + r]);
+      for (int v = 0; v < W; ++v) top = fmaxf(top, red_ref[v * ROWS + r]);
       float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float rw = red_ref[w * ROWS + r];
-        const float f = rw == -INFINITY ? 0.0f : exp2f(rw - top);
-        const float4 v = *reinterpret_cast<const float4 *>(red + (w * ROWS + r) * DIM + dim);
-        sum += red_l[w * ROWS + r] * f;
-        acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
+      for (int v = 0; v < W; ++v) {
+        const float rw = red_ref[v * ROWS + r];
+        const float f = rw == -INFINITY ? 0.0f : exp2_fast(rw - top);
+        const float4 u = *reinterpret_cast<const float4 *>(red + (v * ROWS + r) * DIM + dim);
+        sum = fmaf(red_l[v * ROWS + r], f, sum);
+        acc[0] = fmaf(u.x, f, acc[0]), acc[1] = fmaf(u.y, f, acc[1]);
+        acc[2] = fmaf(u.z, f, acc[2]), acc[3] = fmaf(u.w, f, acc[3]);
       }
       if (whole) {
-        const int64_t rr = rb * ROWS + r, i = (uint32_t)rr / (uint32_t)a.group;
-        if (i < seq.n)
-          finish4<IO>(a, seq.start + i, head * a.group + (int)(rr - i * a.group), dim, top, sum, acc, DIM);
+        const int rr = rb * ROWS + r, i = (int)((uint32_t)rr / (uint32_t)a.group);
+        if (i < seq.n) finish4<IO>(a, seq.start + i, head * a.group + rr - i * a.group, dim, top, sum, acc, DIM);
       } else {
-        *reinterpret_cast<float4 *>(slot + r * DIM + dim) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (dim == 0) slot[ROWS * DIM + r] = top, slot[ROWS * DIM + ROWS + r] = sum;
+        *reinterpret_cast<float4 *>(part + r * DIM + dim) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (dim == 0) part[ROWS * DIM + r] = top, part[ROWS * DIM + ROWS + r] = sum;
       }
     }
     if (!whole) {
       __threadfence();
       __syncthreads();
-      if (tid == 0) {
-        const int32_t parts = (int32_t)(last_share - first_cta + 1);
-        last_cta = atomicAdd(&a.arrive[first_cta], 1) == parts - 1;
-        if (last_cta) a.arrive[first_cta] = 0;
-      }
+      if (tid == 0) last_cta = arrive(a, w);
       __syncthreads();
       if (last_cta) {
         __threadfence();
         for (int x = tid; x < ROWS * DIM / 4; x += kAttnThreads) {
           const int r = x / (DIM / 4), dim = x % (DIM / 4) * 4;
-          const int64_t rr = rb * ROWS + r, i = (uint32_t)rr / (uint32_t)a.group;
+          const int rr = rb * ROWS + r, i = (int)((uint32_t)rr / (uint32_t)a.group);
           if (i >= seq.n) continue;
           float top = -INFINITY;
-          for (int64_t c = first_cta; c <= last_share; ++c)
-            top = fmaxf(top, __ldcg(part_slot<ROWS, DIM>(a, c, first_cta) + ROWS * DIM + r));
+#pragma unroll 4
+          for (int c = first; c <= last; ++c) top = fmaxf(top, __ldcg(part_slot<ROWS, DIM>(a, c, first) + ROWS * DIM + r));
           float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-          for (int64_t c = first_cta; c <= last_share; ++c) {
-            const float *p = part_slot<ROWS, DIM>(a, c, first_cta);
+#pragma unroll 4
+          for (int c = first; c <= last; ++c) {
+            const float *p = part_slot<ROWS, DIM>(a, c, first);
             const float rw = __ldcg(p + ROWS * DIM + r);
-            const float f = rw == -INFINITY ? 0.0f : exp2f(rw - top);
+            const float f = rw == -INFINITY ? 0.0f : exp2_fast(rw - top);
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + r * DIM + dim));
-            sum += __ldcg(p + ROWS * DIM + ROWS + r) * f;
-            acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
+            sum = fmaf(__ldcg(p + ROWS * DIM + ROWS + r), f, sum);
+            acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]);
+            acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
           }
-          finish4<IO>(a, seq.start + i, head * a.group + (int)(rr - i * a.group), dim, top, sum, acc, DIM);
+          finish4<IO>(a, seq.start + i, head * a.group + rr - i * a.group, dim, top, sum, acc, DIM);
         }
       }
     }
+    // the next item's copies write where these sums lay
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
   } while (w.next(a));
 }
@@ -504,8 +532,9 @@ cudaError_t launch_dims(const AttnArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
+// two slots a CTA
 size_t attn_workspace_bytes(int sm_count, int nb) {
-  return (size_t)sm_count * kAttnCtasPerSm * 2 * kAttnMaxRows * (nb * 32 + 2) * sizeof(float);
+  return (size_t)sm_count * kAttnCtasPerSm * 2 * 16 * (nb * 32 + 2) * sizeof(float);
 }
 size_t attn_counter_bytes(int sm_count) { return (size_t)sm_count * kAttnCtasPerSm * sizeof(int32_t); }
 

@@ -82,6 +82,23 @@ __device__ __forceinline__ void store_row4(IO *p, bool vec, const float (&x)[4])
   }
 }
 
+// mbar_wait for waits that are short as a rule: the error flag lies in global
+// memory, so it and the clock are looked at every 64th try only.
+__device__ __forceinline__ bool brief_wait(uint64_t *bar, uint32_t parity, const AttnArgs &a, int code) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 63u) == 0u) {
+      if (*(volatile int32_t *)a.err != 0) return false;  // another role already gave up
+      if (clock64() - t0 > (1ll << a.wait_shift)) {
+        atomicCAS(a.err, 0, code);
+        return false;
+      }
+    }
+  }
+}
+
 // a / b for non-negative a, which seldom need 64 bits.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
@@ -131,11 +148,11 @@ __device__ __forceinline__ int row_blocks(const AttnArgs &a, const SeqRows &s) {
   return (int)(((uint32_t)(s.n * a.group) + ROWS - 1) / ROWS);
 }
 
-// A CTA's walk over its share of the work.  Items are (sequence, key head, row
+// The walk of a CTA or a warp over its share of the work.  Items are (sequence, key head, row
 // block), in that order; an item counts HEAD units for its beginning and end
 // and one for each of its key tiles.  All items' units in a row are cut into
-// equal shares, one a CTA, so ragged batches load every SM alike and a long
-// sequence is split over all of them.
+// equal shares, one a CTA (or warp), so ragged batches load every SM alike and
+// a long sequence is split over all of them.
 template <int ROWS, int KEYS, int HEAD>
 struct AttnWalk {
   int64_t unit, item_begin, end, share;
@@ -164,15 +181,15 @@ struct AttnWalk {
     return v;
   }
 
-  // Every thread of the CTA; false where no work is left for it.  Sequences are
-  // weighed THREADS at a time: by a thread each where they have a row block or
-  // two, by a warp each where they have many.
+  // Finds share `index` of `count` (the same for a warp's threads; every thread of
+  // the CTA takes part); false where it is empty.  Sequences are weighed THREADS
+  // at a time: by a thread each where they have a row block or two, by a warp
+  // each where they have many.
   template <int THREADS>
-  __device__ bool begin(const AttnArgs &a, int64_t min_share) {
+  __device__ bool begin(const AttnArgs &a, int64_t min_share, int index, int count) {
     constexpr int WARPS = THREADS / 32;
     __shared__ int64_t scratch[WARPS];
-    __shared__ int64_t weight[THREADS];
-    __shared__ int64_t found[2];
+    __shared__ int64_t weight[THREADS], before_of[THREADS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool wide = a.r.tokens * a.group > 2 * ROWS * a.r.sequences;
     auto weigh = [&](int64_t b0) {  // units of sequence b0 + tid
@@ -191,46 +208,55 @@ struct AttnWalk {
       __syncthreads();
       return mine;
     };
+    // sums over the warps before this one, and over all
+    auto block_scan = [&](int64_t up, int64_t *all) {
+      if (lane == 31) scratch[warp] = up;
+      __syncthreads();
+      int64_t sum = 0, below = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == warp) below = sum;
+        sum += scratch[w];
+      }
+      __syncthreads();
+      *all = sum;
+      return below;
+    };
     const int64_t mine = weigh(0);
     int64_t total = mine;
     for (int64_t b0 = THREADS; b0 < a.r.sequences; b0 += THREADS) total += weigh(b0);
-    total = warp_sum(total);
-    if (lane == 0) scratch[warp] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += scratch[w];
-    __syncthreads();
-    share = quotient(total + gridDim.x - 1, gridDim.x);
+    block_scan(warp_sum(total), &total);
+    share = quotient(total + count - 1, count);
     if (share < min_share) share = min_share;
-    unit = (int64_t)blockIdx.x * share;
+    unit = (int64_t)index * share;
     end = unit + share < total ? unit + share : total;
-    if (unit >= total) return false;
-    int64_t before = 0;  // the sequence that holds `unit`, and the units before it
+    int64_t per_head = 1, before = 0;
+    b = -1;
     for (int64_t b0 = 0; b0 < a.r.sequences; b0 += THREADS) {
       const int64_t v = b0 == 0 ? mine : weigh(b0);
-      int64_t up = warp_scan(v, lane);
-      if (lane == 31) scratch[warp] = up;
+      const int64_t up = warp_scan(v, lane);
+      int64_t all;
+      const int64_t below = block_scan(up, &all);
+      weight[tid] = v;
+      before_of[tid] = before + below + up - v;
       __syncthreads();
-      int64_t all = 0;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) up += scratch[w];
-        all += scratch[w];
-      }
-      const int64_t first = before + up - v;
-      if (unit >= first && unit < first + v) {
-        found[0] = b0 + tid, found[1] = first;
-        weight[0] = quotient(v, a.c.kv_heads);
-      }
+      if (b < 0 && unit >= before && unit < before + all)  // the sequence that holds `unit`
+        for (int i = 0; i < WARPS; ++i) {
+          const int64_t at = before_of[i * 32 + lane], n = weight[i * 32 + lane];
+          const uint32_t hit = __ballot_sync(0xffffffffu, unit >= at && unit < at + n);
+          if (hit) {
+            const int x = i * 32 + __ffs(hit) - 1;
+            b = (int)(b0 + x);
+            item_begin = before_of[x];
+            per_head = quotient(weight[x], a.c.kv_heads);
+            break;
+          }
+        }
       before += all;
       __syncthreads();
-      if (before > unit) break;
     }
-    b = (int)found[0];
-    item_begin = found[1];
+    if (unit >= total) return false;
     seq = seq_rows(a, b);
-    const int64_t per_head = weight[0];
     head = (int)quotient(unit - item_begin, per_head);
     item_begin += head * per_head;
     // the row block that holds `unit`: 32 at a time
@@ -252,7 +278,7 @@ struct AttnWalk {
     return true;
   }
 
-  // This CTA's part of the current item: units, and tiles [first_tile(), last_tile()).
+  // This share's part of the current item: units, and tiles [first_tile(), last_tile()).
   __device__ int units() const { return cost(tiles); }
   __device__ int take() const {
     const int left = units() - (int)(unit - item_begin);
@@ -265,8 +291,8 @@ struct AttnWalk {
   __device__ int first_tile() const { return tile_at(unit); }
   __device__ int last_tile() const { return tile_at(unit + take()); }
   __device__ bool whole() const { return take() == units(); }
-  __device__ int first_cta() const { return (int)quotient(item_begin, share); }
-  __device__ int last_cta() const { return (int)quotient(item_begin + units() - 1, share); }
+  __device__ int first_share() const { return (int)quotient(item_begin, share); }
+  __device__ int last_share() const { return (int)quotient(item_begin + units() - 1, share); }
 
   __device__ bool next(const AttnArgs &a) {
     const int t = take();
@@ -286,12 +312,20 @@ struct AttnWalk {
   }
 };
 
-// An item that several CTAs share: the first of them keeps its part in its
-// slot 1, every other in its slot 0; the last to arrive joins the parts in the
-// order of the CTAs, so that the order of arrival changes nothing.
+// An item in several shares: the first keeps its part in its slot 1, every
+// other in its slot 0; the last to arrive joins the parts in the order of the
+// shares, so that the order of arrival changes nothing.
 template <int ROWS, int DIM>
-__device__ __forceinline__ float *part_slot(const AttnArgs &a, int64_t cta, int64_t first_cta) {
-  return a.partial + (cta * 2 + (cta == first_cta)) * (ROWS * (DIM + 2));
+__device__ __forceinline__ float *part_slot(const AttnArgs &a, int share, int first) {
+  return a.partial + ((int64_t)share * 2 + (share == first)) * (ROWS * (DIM + 2));
+}
+// Counts a part; whether it was the last.
+template <typename Walk>
+__device__ __forceinline__ bool arrive(const AttnArgs &a, const Walk &w) {
+  const int first = w.first_share();
+  const bool last = atomicAdd(&a.arrive[first], 1) == w.last_share() - first;
+  if (last) a.arrive[first] = 0;
+  return last;
 }
 
 // What a row's sums, which stand for 2^ref times their value, are multiplied by

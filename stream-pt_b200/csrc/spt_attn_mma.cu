@@ -139,23 +139,7 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// mbar_wait for waits that are short as a rule: the error flag lies in global
-// memory, so it and the clock are looked at every 64th try only.
-__device__ __forceinline__ bool brief_wait(uint64_t *bar, uint32_t parity, const AttnArgs &a, int code) {
-  if (mbar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try(bar, parity)) return true;
-    if ((i & 63u) == 0u) {
-      if (*(volatile int32_t *)a.err != 0) return false;  // another role already gave up
-      if (clock64() - t0 > (1ll << a.wait_shift)) {
-        atomicCAS(a.err, 0, code);
-        return false;
-      }
-    }
-  }
-}
-// The same for a whole warp, which passes or gives up together.
+// brief_wait for a whole warp, which passes or gives up together.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, const AttnArgs &a, int code) {
   return __all_sync(0xffffffffu, brief_wait(bar, parity, a, code));
 }
@@ -488,15 +472,6 @@ __device__ __forceinline__ bool issue(const AttnArgs &a, MmaCta<NB, IO> &s, uint
   return true;
 }
 
-// Counts this CTA's part of an item; whether it was the last.
-template <int NB, typename IO>
-__device__ __forceinline__ bool arrive(const AttnArgs &a, const MmaWalk<NB, IO> &w) {
-  const int first = w.first_cta();
-  const bool last = atomicAdd(&a.arrive[first], 1) == w.last_cta() - first;
-  if (last) a.arrive[first] = 0;
-  return last;
-}
-
 // The softmax warps: thread = row.  `arrived`: the current item's part is
 // counted.
 template <int NB, typename IO>
@@ -701,7 +676,7 @@ __device__ __forceinline__ bool softmax(const AttnArgs &a, MmaCta<NB, IO> &s, ui
     float end_ref = fresh && l == 0.0f ? -INFINITY : ref;
     bool write = true;
     if (!w.whole()) {
-      const int first_cta = w.first_cta(), last_cta = w.last_cta();
+      const int first_cta = w.first_share(), last_cta = w.last_share();
       float *slot = part_slot<ROWS, DIM>(a, blockIdx.x, first_cta);
 #pragma unroll
       for (int x = 0; x < DIM / 2; x += 2)  // column groups first: neighbouring rows lie side by side
@@ -713,7 +688,7 @@ __device__ __forceinline__ bool softmax(const AttnArgs &a, MmaCta<NB, IO> &s, ui
       if (lane == 0) mbar_arrive(&s.meet);
       if (!warp_wait(&s.meet, parts & 1u, a, 41)) return false;
       if (row == 0) {
-        s.last = arrive<NB, IO>(a, w);
+        s.last = arrive(a, w);
         mbar_arrive(&s.told);
       }
       arrived = true;
@@ -793,7 +768,7 @@ __global__ void __launch_bounds__(MmaTile<NB, IO>::kThreads, 1) k_attn_mma(const
   pdl_wait();
   pdl_trigger();
   MmaWalk<NB, IO> w;
-  if (!w.template begin<T::kThreads>(a, kMmaMinTiles)) return;
+  if (!w.template begin<T::kThreads>(a, kMmaMinTiles, blockIdx.x, gridDim.x)) return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < T::kRaw; ++i) {
       mbar_init(&s.raw_full[i], 1);
@@ -837,7 +812,7 @@ __global__ void __launch_bounds__(MmaTile<NB, IO>::kThreads, 1) k_attn_mma(const
     if (!softmax<NB, IO>(a, s, smem, w, warp, lane, arrived) && threadIdx.x == 0) {
       // a wait gave up: the parts that are left still count, so that the counters end at zero
       do {
-        if (!arrived && !w.whole()) arrive<NB, IO>(a, w);
+        if (!arrived && !w.whole()) arrive(a, w);
         arrived = false;
       } while (w.next(a));
     }
