@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "spt_device.cuh"
 #include "spt_internal.cuh"
 #include "spt_kv.cuh"
@@ -11,28 +13,49 @@
 namespace spt {
 namespace {
 
-constexpr int kKvThreads = 256;
-constexpr int kKvSpan = 8;  // values a thread quantises; four threads share a block
+constexpr int kKvThreads = 256, kKvWarps = kKvThreads / 32;
 
-// Sequence and position of a new row; false where the row belongs to none or
-// its position has no place in the table.
-__device__ __forceinline__ bool kv_locate(const KvRows &r, int64_t row, int64_t places, int64_t *seq, int64_t *pos) {
+// A warp's work: the new rows of a sequence that fall into one 16-token tile,
+// for one head, keys or values.  Tiles are numbered so that a binary search
+// finds them: sequence b has the slots from offsets[b] / 16 + 2 b on, which are
+// as many as its rows can need wherever they start (n / 16 + 2).
+struct KvUnit {
+  int seq, tile, lo, hi;  // tokens [lo, hi) of the tile are new
+  int row;                // of token lo
+};
+inline int64_t kv_slots(const KvRows &r) {
+  return r.offsets ? r.tokens / kKvTile + 2 * r.sequences + 1 : r.sequences < r.tokens ? r.sequences : r.tokens;
+}
+__device__ __forceinline__ bool kv_unit(const KvRows &r, int64_t slot, KvUnit *u) {
+  int len, start, n, first;  // first: the slot of the sequence's first tile, less `slot`
   if (!r.offsets) {
-    if (row >= r.sequences) return false;
-    *seq = row;
-    *pos = (int64_t)r.lengths[row] - 1;
+    if (slot >= r.sequences || slot >= r.tokens) return false;
+    u->seq = (int)slot;
+    len = r.lengths[slot], start = (int)slot, n = 1, first = 0;
   } else {
-    if (row < r.offsets[0] || row >= r.offsets[r.sequences]) return false;
-    int64_t lo = 0, hi = r.sequences - 1;  // the first sequence whose rows end behind `row`
+    int64_t lo = 0, hi = r.sequences - 1;  // the last sequence whose slots start at or before `slot`
     while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (r.offsets[mid + 1] > row) hi = mid;
-      else lo = mid + 1;
+      const int64_t mid = (lo + hi + 1) >> 1;
+      if (r.offsets[mid] / kKvTile + 2 * mid <= slot) lo = mid;
+      else hi = mid - 1;
     }
-    *seq = lo;
-    *pos = (int64_t)r.lengths[lo] - r.offsets[lo + 1] + row;
+    u->seq = (int)lo;
+    len = r.lengths[lo], start = r.offsets[lo];
+    const int end = r.offsets[lo + 1];
+    if (start < 0 || end > r.tokens || end <= start) return false;
+    n = end - start;
+    const int64_t past = slot - (start / kKvTile + 2 * lo);
+    if (past < 0 || past > n / kKvTile + 1) return false;
+    first = (int)past;
   }
-  return *pos >= 0 && *pos < places;
+  const int64_t pos0 = (int64_t)len - n;  // (rows before position 0 have no place)
+  const int p0 = pos0 > 0 ? (int)pos0 : 0;
+  u->tile = p0 / kKvTile + first;
+  const int64_t from = (int64_t)u->tile * kKvTile;
+  u->lo = (int)(from > p0 ? from : p0);
+  u->hi = (int)(from + kKvTile < len ? from + kKvTile : len);
+  u->row = start + (int)(u->lo - pos0);
+  return u->lo < u->hi;
 }
 
 template <typename T>
@@ -52,70 +75,92 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *p, float (&x)[kKvSpan]) {
+// N consecutive elements, 4 or 8; VEC: the row starts on 16 bytes.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_n(const T *p, float (&x)[N]) {
   if constexpr (VEC) {
-    constexpr int W = sizeof(T) * kKvSpan / 16;
-    uint4 w[W];
+    constexpr int B = N * (int)sizeof(T);  // 8, 16 or 32 bytes
+    using W = typename std::conditional<B == 8, uint2, uint4>::type;
+    W w[B / sizeof(W)];
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    for (int i = 0; i < B / (int)sizeof(W); ++i) w[i] = __ldcs(reinterpret_cast<const W *>(p) + i);
     const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
-    for (int i = 0; i < kKvSpan; ++i) x[i] = to_float<T>(e[i]);
+    for (int i = 0; i < N; ++i) x[i] = to_float<T>(e[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kKvSpan; ++i) x[i] = to_float<T>(p[i]);
+    for (int i = 0; i < N; ++i) x[i] = to_float<T>(p[i]);
   }
 }
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T *p, const float (&x)[kKvSpan]) {
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
   if constexpr (VEC) {
-    constexpr int W = sizeof(T) * kKvSpan / 16;
-    uint4 w[W];
+    constexpr int B = N * (int)sizeof(T);
+    using W = typename std::conditional<B == 8, uint2, uint4>::type;
+    W w[B / sizeof(W)];
     T *e = reinterpret_cast<T *>(w);
 #pragma unroll
-    for (int i = 0; i < kKvSpan; ++i) e[i] = from_float<T>(x[i]);
+    for (int i = 0; i < N; ++i) e[i] = from_float<T>(x[i]);
 #pragma unroll
-    for (int i = 0; i < W; ++i) __stcs(reinterpret_cast<uint4 *>(p) + i, w[i]);
+    for (int i = 0; i < B / (int)sizeof(W); ++i) __stcs(reinterpret_cast<W *>(p) + i, w[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kKvSpan; ++i) p[i] = from_float<T>(x[i]);
+    for (int i = 0; i < N; ++i) p[i] = from_float<T>(x[i]);
   }
 }
 
-// Scale and codes of a block held by four neighbouring lanes, eight values
-// each; nibble i of the result is value i of this lane.
-__device__ __forceinline__ uint32_t kv_quantise(const float (&x)[kKvSpan], int quarter, __half *scale) {
+// Scale and codes of a block whose 32 values lie with 32 / N lanes, N each,
+// STEP lanes apart; nibble i of the result is value i of this lane, `part` the
+// lane's place in the block.
+template <int N, int STEP>
+__device__ __forceinline__ uint32_t kv_quantise(const float (&x)[N], int part, __half *scale) {
   float top = x[0];
-  bool nan = isnan(x[0]);
-  int at = 0;
+  int at = 0, nan = isnan(x[0]);
 #pragma unroll
-  for (int i = 1; i < kKvSpan; ++i) {
+  for (int i = 1; i < N; ++i) {
     nan |= isnan(x[i]);
     if (fabsf(x[i]) > fabsf(top)) top = x[i], at = i;
   }
-  at += quarter * kKvSpan;
-  int any = nan;
+  at += part * N;
 #pragma unroll
-  for (int m = 1; m < 4; m <<= 1) {
+  for (int m = STEP; m < STEP * 32 / N; m <<= 1) {
     const float o = __shfl_xor_sync(0xffffffffu, top, m);
     const int oat = __shfl_xor_sync(0xffffffffu, at, m);
-    any |= __shfl_xor_sync(0xffffffffu, any, m);
+    nan |= __shfl_xor_sync(0xffffffffu, nan, m);
     if (fabsf(o) > fabsf(top) || (fabsf(o) == fabsf(top) && oat < at)) top = o, at = oat;
   }
   const float wide = fminf(fmaxf(top * -0.125f, -65504.0f), 65504.0f);
-  const __half d = any ? __ushort_as_half(0x7fff) : __float2half_rn(wide);
+  const __half d = nan ? __ushort_as_half(0x7fff) : __float2half_rn(wide);
   *scale = d;
   const float step = __half2float(d);
-  uint32_t codes = 0;
+  const float inv = step != 0.0f && !nan ? __fdiv_rn(1.0f, step) : 0.0f;
+  // x * inv is within 8.5 * 2^-23 of the quotient: its rounding is the
+  // quotient's unless it lies that near a half.  Adding 1.5 * 2^23 rounds to
+  // even, and leaves the integer in the low bits.
+  constexpr float kMagic = 12582912.0f;
+  float k[N], near = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kKvSpan; ++i) {
-    const float q = step != 0.0f ? rintf(__fdiv_rn(x[i], step)) : 0.0f;
-    const int n = any ? 8 : (int)fminf(fmaxf(q, -8.0f), 7.0f) + 8;
-    codes |= (uint32_t)n << (4 * i);
+  for (int i = 0; i < N; ++i) {
+    const float q = fminf(fmaxf(__fmul_rn(x[i], inv), -8.0f), 7.0f);  // (a NaN becomes -8; its block has no codes)
+    k[i] = __fadd_rn(q, kMagic);
+    near = fmaxf(near, fabsf(__fsub_rn(q, __fsub_rn(k[i], kMagic))));
   }
-  return codes;
+  uint32_t codes = 0;
+  if (__any_sync(0xffffffffu, near > 0.499996f)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      // the remainder x - n d is exact; beyond half a step, or on it with an odd n, the next n is right
+      float n = __fsub_rn(k[i], kMagic);
+      const float e = __fmaf_rn(-n, step, x[i]);
+      const float over = __fsub_rn(2.0f * fabsf(e), fabsf(step));
+      if (over > 0.0f || (over == 0.0f && (__float_as_uint(k[i]) & 1u)))
+        n = __fadd_rn(n, (e < 0.0f) == (step < 0.0f) ? 1.0f : -1.0f);
+      k[i] = __fadd_rn(fminf(fmaxf(n, -8.0f), 7.0f), kMagic);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) codes |= ((__float_as_uint(k[i]) + 8u) & 15u) << (4 * i);
+  return nan || step == 0.0f ? 0x88888888u >> (32 - 4 * N) : codes;
 }
 
 struct KvMove {
@@ -124,109 +169,190 @@ struct KvMove {
   const void *src[2];
   void *dst[2];
   int64_t stride[2];
+  int64_t units;
 };
 
-// One thread: eight consecutive values of one row's key or value (blockIdx.y).
-// Bound by memory: each row is read once and 9/16 byte a value written.
-template <typename T, bool VEC>
+// This warp's unit and its tile's record; null where there is nothing to do.
+__device__ __forceinline__ uint8_t *kv_record(const KvMove &a, KvUnit *u, int *head) {
+  const int64_t id = (int64_t)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
+  if (id >= a.units) return nullptr;
+  const int64_t slot = (uint32_t)id / (uint32_t)a.c.kv_heads;
+  *head = (int)(id - slot * a.c.kv_heads);
+  if (!kv_unit(a.r, slot, u)) return nullptr;
+  const int tiles = a.c.page_tokens / kKvTile, entry = u->tile / tiles;
+  if (entry >= a.r.max_pages) return nullptr;
+  const int64_t page = a.r.table[u->seq * a.r.max_pages + entry];
+  if (page < 0 || page >= a.c.pages) return nullptr;
+  return a.c.base + kv_tile_offset(a.c, page, *head, (u->tile - entry * tiles) * kKvTile);
+}
+
+// Bound by memory: rows are read once and the records written once.  A tile
+// whose 16 tokens are all new leaves as 16-byte pieces; else every token's
+// codes are stored by themselves.  Lane 4 g + t holds, of keys, tokens g and
+// g + 8, dims 8 t on of each block; of values, tokens 2 t, 2 t + 1, 2 t + 8 and
+// 2 t + 9, dims 4 g on: the words that the layout gives it.
+template <typename T, int NB, bool VEC>
 __global__ void __launch_bounds__(kKvThreads) k_kv_append(const KvMove a) {
   pdl_wait();
   pdl_trigger();
-  const KvLayer &c = a.c;
-  const int per_row = c.kv_heads * c.nb * 4;
-  const int64_t id = (int64_t)blockIdx.x * kKvThreads + threadIdx.x;
-  const int64_t row = id / per_row;
+  KvUnit u;
+  int head;
+  uint8_t *const rec = kv_record(a, &u, &head);
+  if (!rec) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const bool value = blockIdx.y != 0;
-  int64_t seq = 0, pos = 0;
-  bool live = row < a.r.tokens && kv_locate(a.r, row, a.r.max_pages * c.page_tokens, &seq, &pos);
-  int64_t page = 0;
-  if (live) {
-    page = a.r.table[seq * a.r.max_pages + pos / c.page_tokens];
-    live = page >= 0 && page < c.pages;
-  }
-  const int part = (int)(id - row * per_row);
-  const int head = part / (c.nb * 4), block = part / 4 % c.nb, quarter = part & 3;
-  float x[kKvSpan] = {};
-  if (live)
-    load8<T, VEC>(static_cast<const T *>(a.src[value]) + row * a.stride[value] +
-                      (int64_t)head * c.nb * kKvBlock + block * kKvBlock + quarter * kKvSpan, x);
-  __half d;
-  const uint32_t codes = kv_quantise(x, quarter, &d);
-  if (!live) return;
-  const int place = (int)(pos % c.page_tokens), token = place % kKvTile;
-  uint8_t *tile = c.base + kv_tile_offset(c, page, head, place);
+  const int first = u.lo - u.tile * kKvTile, end = u.hi - u.tile * kKvTile;  // new tokens of the tile
+  const bool all = end - first == kKvTile;
+  const int64_t stride = value ? a.stride[1] : a.stride[0];
+  const T *src = static_cast<const T *>(value ? a.src[1] : a.src[0]) + (int64_t)(u.row - first) * stride + head * (NB * 32);
+  uint32_t w[NB][2];
   if (!value) {
-    *reinterpret_cast<uint32_t *>(tile + kv_word(c.nb, block, (token & 7) * 4 + quarter, token >> 3)) = codes;
+    float x[NB][2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int token = g + 8 * h;
+        if (token >= first && token < end) load_n<T, 8, VEC>(src + token * stride + b * 32 + t * 8, x[b][h]);
+        else
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[b][h][i] = 0.0f;
+      }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int token = g + 8 * h;
+        __half d;
+        w[b][h] = kv_quantise<8, 1>(x[b][h], t, &d);
+        if (token < first || token >= end) continue;
+        if (t == 0) *reinterpret_cast<__half *>(rec + kv_key_scales(NB) + kv_scale(NB, b, token)) = d;
+        if (!all) *reinterpret_cast<uint32_t *>(rec + kv_word(NB, b, lane, h)) = w[b][h];
+      }
   } else {
-    uint8_t *v = tile + kv_value_codes(c.nb) + 2 * (token & 1);
-    const int t = (token & 7) >> 1, h = token >> 3;
-    *reinterpret_cast<uint16_t *>(v + kv_word(c.nb, block, (2 * quarter) * 4 + t, h)) = (uint16_t)codes;
-    *reinterpret_cast<uint16_t *>(v + kv_word(c.nb, block, (2 * quarter + 1) * 4 + t, h)) = (uint16_t)(codes >> 16);
+    float x[NB][4][4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int token = 2 * t + (y & 1) + 8 * (y >> 1);
+        if (token >= first && token < end) load_n<T, 4, VEC>(src + token * stride + b * 32 + g * 4, x[b][y]);
+        else
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[b][y][i] = 0.0f;
+      }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      w[b][0] = w[b][1] = 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int token = 2 * t + (y & 1) + 8 * (y >> 1);
+        __half d;
+        const uint32_t codes = kv_quantise<4, 4>(x[b][y], g, &d);
+        w[b][y >> 1] |= codes << (16 * (y & 1));
+        if (token < first || token >= end) continue;
+        if (g == 0) *reinterpret_cast<__half *>(rec + kv_value_scales(NB) + kv_scale(NB, b, token)) = d;
+        if (!all)
+          *reinterpret_cast<uint16_t *>(rec + kv_value_codes(NB) + kv_word(NB, b, lane, y >> 1) + 2 * (y & 1)) = (uint16_t)codes;
+      }
+    }
   }
-  if (quarter == 0)
-    *reinterpret_cast<__half *>(tile + (value ? kv_value_scales(c.nb) : kv_key_scales(c.nb)) +
-                                kv_scale(c.nb, block, token)) = d;
+  if (!all) return;
+  uint8_t *to = rec + (value ? kv_value_codes(NB) : 0);
+#pragma unroll
+  for (int b = 0; b + 1 < NB; b += 2)
+    *reinterpret_cast<uint4 *>(to + kv_word(NB, b, lane, 0)) = make_uint4(w[b][0], w[b][1], w[b + 1][0], w[b + 1][1]);
+  if constexpr (NB % 2 == 1)
+    *reinterpret_cast<uint2 *>(to + kv_word(NB, NB - 1, lane, 0)) = make_uint2(w[NB - 1][0], w[NB - 1][1]);
 }
 
-template <typename T, bool VEC>
+template <typename T, int NB, bool VEC>
 __global__ void __launch_bounds__(kKvThreads) k_kv_read(const KvMove a) {
   pdl_wait();
   pdl_trigger();
-  const KvLayer &c = a.c;
-  const int per_row = c.kv_heads * c.nb * 4;
-  const int64_t id = (int64_t)blockIdx.x * kKvThreads + threadIdx.x;
-  const int64_t row = id / per_row;
   const bool value = blockIdx.y != 0;
-  if (!a.dst[value] || row >= a.r.tokens) return;
-  int64_t seq, pos;
-  if (!kv_locate(a.r, row, a.r.max_pages * c.page_tokens, &seq, &pos)) return;
-  const int64_t page = a.r.table[seq * a.r.max_pages + pos / c.page_tokens];
-  if (page < 0 || page >= c.pages) return;
-  const int part = (int)(id - row * per_row);
-  const int head = part / (c.nb * 4), block = part / 4 % c.nb, quarter = part & 3;
-  const int place = (int)(pos % c.page_tokens), token = place % kKvTile;
-  const uint8_t *tile = c.base + kv_tile_offset(c, page, head, place);
-  uint32_t codes;
-  if (!value) {
-    codes = *reinterpret_cast<const uint32_t *>(tile + kv_word(c.nb, block, (token & 7) * 4 + quarter, token >> 3));
-  } else {
-    const uint8_t *v = tile + kv_value_codes(c.nb) + 2 * (token & 1);
-    const int t = (token & 7) >> 1, h = token >> 3;
-    codes = *reinterpret_cast<const uint16_t *>(v + kv_word(c.nb, block, (2 * quarter) * 4 + t, h)) |
-            (uint32_t) * reinterpret_cast<const uint16_t *>(v + kv_word(c.nb, block, (2 * quarter + 1) * 4 + t, h)) << 16;
-  }
-  const float d = __half2float(*reinterpret_cast<const __half *>(
-      tile + (value ? kv_value_scales(c.nb) : kv_key_scales(c.nb)) + kv_scale(c.nb, block, token)));
-  float x[kKvSpan];
+  void *const out = value ? a.dst[1] : a.dst[0];
+  KvUnit u;
+  int head;
+  const uint8_t *const rec = out ? kv_record(a, &u, &head) : nullptr;
+  if (!rec) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int first = u.lo - u.tile * kKvTile, end = u.hi - u.tile * kKvTile;
+  const int64_t stride = value ? a.stride[1] : a.stride[0];
+  T *dst = static_cast<T *>(out) + (int64_t)(u.row - first) * stride + head * (NB * 32);
+  uint2 w[NB], s[NB];
 #pragma unroll
-  for (int i = 0; i < kKvSpan; ++i) x[i] = (float)((int)(codes >> (4 * i) & 15u) - 8) * d;
-  store8<T, VEC>(static_cast<T *>(a.dst[value]) + row * a.stride[value] + (int64_t)head * c.nb * kKvBlock +
-                     block * kKvBlock + quarter * kKvSpan, x);
+  for (int b = 0; b < NB; ++b) {
+    w[b] = *reinterpret_cast<const uint2 *>(rec + (value ? kv_value_codes(NB) : 0) + kv_word(NB, b, lane, 0));
+    // the four scales of this lane's tokens: 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of values, those of g & ~1 for keys
+    s[b] = *reinterpret_cast<const uint2 *>(rec + (value ? kv_value_scales(NB) : kv_key_scales(NB)) +
+                                               (value ? t : g >> 1) * NB * 8 + b * 8);
+  }
+  auto scale_of = [&](int b, int h, int odd) {
+    const uint32_t pair = h ? s[b].y : s[b].x;
+    return __half2float(__ushort_as_half((unsigned short)(odd ? pair >> 16 : pair)));
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t word = h ? w[b].y : w[b].x;
+      if (!value) {
+        const int token = g + 8 * h;
+        if (token < first || token >= end) continue;
+        const float d = scale_of(b, h, g & 1);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)((int)(word >> (4 * i) & 15u) - 8) * d;
+        store_n<T, 8, VEC>(dst + token * stride + b * 32 + t * 8, x);
+      } else {
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+          const int token = 2 * t + odd + 8 * h;
+          if (token < first || token >= end) continue;
+          const float d = scale_of(b, h, odd);
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = (float)((int)(word >> (16 * odd + 4 * i) & 15u) - 8) * d;
+          store_n<T, 4, VEC>(dst + token * stride + b * 32 + g * 4, x);
+        }
+      }
+    }
 }
 
-// 16-byte accesses need rows that start on 16 bytes (a head's and a thread's
-// share are multiples of 16 bytes in every type).
+// 16-byte accesses need rows that start on 16 bytes (a head's share is a
+// multiple of 64 bytes in every type).
 bool vectors(const void *p, int64_t stride, int size) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * size) % 16 == 0;
 }
 
-template <typename T>
-cudaError_t launch_move(const KvMove &a, bool append, cudaStream_t stream) {
-  const int64_t threads = a.r.tokens * a.c.kv_heads * a.c.nb * 4;
-  const int64_t blocks = (threads + kKvThreads - 1) / kKvThreads;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)blocks, 2), block(kKvThreads);
+template <typename T, int NB>
+cudaError_t launch_blocks(const KvMove &a, bool append, cudaStream_t stream) {
+  const dim3 grid((unsigned)((a.units + kKvWarps - 1) / kKvWarps), 2), block(kKvThreads);
   bool vec = true;
   for (int i = 0; i < 2; ++i) vec = vec && vectors(append ? a.src[i] : a.dst[i], a.stride[i], sizeof(T));
   if (append)
-    return vec ? launch_pdl(k_kv_append<T, true>, grid, block, 0, stream, a)
-               : launch_pdl(k_kv_append<T, false>, grid, block, 0, stream, a);
-  return vec ? launch_pdl(k_kv_read<T, true>, grid, block, 0, stream, a)
-             : launch_pdl(k_kv_read<T, false>, grid, block, 0, stream, a);
+    return vec ? launch_pdl(k_kv_append<T, NB, true>, grid, block, 0, stream, a)
+               : launch_pdl(k_kv_append<T, NB, false>, grid, block, 0, stream, a);
+  return vec ? launch_pdl(k_kv_read<T, NB, true>, grid, block, 0, stream, a)
+             : launch_pdl(k_kv_read<T, NB, false>, grid, block, 0, stream, a);
 }
 
-cudaError_t launch_typed(const KvMove &a, int type, bool append, cudaStream_t stream) {
+template <typename T>
+cudaError_t launch_move(const KvMove &a, bool append, cudaStream_t stream) {
+  switch (a.c.nb) {
+    case 1: return launch_blocks<T, 1>(a, append, stream);
+    case 2: return launch_blocks<T, 2>(a, append, stream);
+    case 3: return launch_blocks<T, 3>(a, append, stream);
+    case 4: return launch_blocks<T, 4>(a, append, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_typed(KvMove a, int type, bool append, cudaStream_t stream) {
   if (a.r.tokens <= 0 || a.r.sequences <= 0) return cudaSuccess;
+  a.units = kv_slots(a.r) * a.c.kv_heads;
+  if (a.units > 0x7fffffffll) return cudaErrorInvalidValue;
   switch (type) {
     case kKvF32: return launch_move<float>(a, append, stream);
     case kKvF16: return launch_move<__half>(a, append, stream);
@@ -282,13 +408,13 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_reorder(uint8_t *pool, int64_
 
 cudaError_t launch_kv_append(const KvLayer &c, const KvRows &r, int type, const void *k, int64_t k_stride,
                              const void *v, int64_t v_stride, cudaStream_t stream) {
-  const KvMove a = {c, r, {k, v}, {nullptr, nullptr}, {k_stride, v_stride}};
+  const KvMove a = {c, r, {k, v}, {nullptr, nullptr}, {k_stride, v_stride}, 0};
   return launch_typed(a, type, true, stream);
 }
 
 cudaError_t launch_kv_read(const KvLayer &c, const KvRows &r, int type, void *k, int64_t k_stride, void *v,
                            int64_t v_stride, cudaStream_t stream) {
-  const KvMove a = {c, r, {nullptr, nullptr}, {k, v}, {k_stride, v_stride}};
+  const KvMove a = {c, r, {nullptr, nullptr}, {k, v}, {k_stride, v_stride}, 0};
   return launch_typed(a, type, false, stream);
 }
 
