@@ -75,10 +75,15 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive elements, 4 or 8; VEC: the row starts on 16 bytes.
+// N consecutive elements, 4 or 8; VEC: they start on as many bytes as they have.
 template <typename T, int N, bool VEC>
 __device__ __forceinline__ void load_n(const T *p, float (&x)[N]) {
-  if constexpr (VEC) {
+  if constexpr (VEC && N * sizeof(T) == 32) {
+    asm("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+        : "l"(p)
+        : "memory");
+  } else if constexpr (VEC) {
     constexpr int B = N * (int)sizeof(T);  // 8, 16 or 32 bytes
     using W = typename std::conditional<B == 8, uint2, uint4>::type;
     W w[B / sizeof(W)];
@@ -94,7 +99,11 @@ __device__ __forceinline__ void load_n(const T *p, float (&x)[N]) {
 }
 template <typename T, int N, bool VEC>
 __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
-  if constexpr (VEC) {
+  if constexpr (VEC && N * sizeof(T) == 32) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                 "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
+  } else if constexpr (VEC) {
     constexpr int B = N * (int)sizeof(T);
     using W = typename std::conditional<B == 8, uint2, uint4>::type;
     W w[B / sizeof(W)];
@@ -109,25 +118,33 @@ __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
   }
 }
 
-// Scale and codes of a block whose 32 values lie with 32 / N lanes, N each,
-// STEP lanes apart; nibble i of the result is value i of this lane, `part` the
-// lane's place in the block.
-template <int N, int STEP>
-__device__ __forceinline__ uint32_t kv_quantise(const float (&x)[N], int part, __half *scale) {
-  float top = x[0];
-  int at = 0, nan = isnan(x[0]);
+// Scale and codes of a block held by four neighbouring lanes, eight values
+// each; nibble i of the result is value i of this lane, `quarter` the lane's
+// place in the block.
+__device__ __forceinline__ uint32_t kv_quantise(const float (&x)[8], int quarter, __half *scale) {
+  constexpr int N = 8;
+  float high = x[0], low = x[0];
+  int nan = isnan(x[0]);
 #pragma unroll
   for (int i = 1; i < N; ++i) {
     nan |= isnan(x[i]);
-    if (fabsf(x[i]) > fabsf(top)) top = x[i], at = i;
+    high = fmaxf(high, x[i]), low = fminf(low, x[i]);
   }
-  at += part * N;
 #pragma unroll
-  for (int m = STEP; m < STEP * 32 / N; m <<= 1) {
-    const float o = __shfl_xor_sync(0xffffffffu, top, m);
-    const int oat = __shfl_xor_sync(0xffffffffu, at, m);
+  for (int m = 1; m < 4; m <<= 1) {
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, m));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, m));
     nan |= __shfl_xor_sync(0xffffffffu, nan, m);
-    if (fabsf(o) > fabsf(top) || (fabsf(o) == fabsf(top) && oat < at)) top = o, at = oat;
+  }
+  float top = high >= -low ? high : low;
+  if (__any_sync(0xffffffffu, high == -low)) {  // both signs have the largest magnitude: the first element that has it
+    int at = 2 * 32;  // twice its place, and one more where it is negative
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i)
+      if (fabsf(x[i]) == high) at = 2 * (quarter * N + i) + (x[i] < 0.0f);
+#pragma unroll
+    for (int m = 1; m < 4; m <<= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, m));
+    if (high == -low) top = at & 1 ? low : high;
   }
   const float wide = fminf(fmaxf(top * -0.125f, -65504.0f), 65504.0f);
   const __half d = nan ? __ushort_as_half(0x7fff) : __float2half_rn(wide);
@@ -186,11 +203,11 @@ __device__ __forceinline__ uint8_t *kv_record(const KvMove &a, KvUnit *u, int *h
   return a.c.base + kv_tile_offset(a.c, page, *head, (u->tile - entry * tiles) * kKvTile);
 }
 
-// Bound by memory: rows are read once and the records written once.  A tile
-// whose 16 tokens are all new leaves as 16-byte pieces; else every token's
-// codes are stored by themselves.  Lane 4 g + t holds, of keys, tokens g and
-// g + 8, dims 8 t on of each block; of values, tokens 2 t, 2 t + 1, 2 t + 8 and
-// 2 t + 9, dims 4 g on: the words that the layout gives it.
+// Bound by memory: rows are read once and the records written once.  Lane 4 g +
+// t quantises dims 8 t on of each block of tokens g and g + 8; that is the
+// keys' layout, and for the values' two lanes' words are exchanged for their
+// halves.  A tile whose 16 tokens are all new leaves as 16-byte pieces; else
+// every token's codes are stored by themselves.
 template <typename T, int NB, bool VEC>
 __global__ void __launch_bounds__(kKvThreads) k_kv_append(const KvMove a) {
   pdl_wait();
@@ -205,65 +222,61 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_append(const KvMove a) {
   const bool all = end - first == kKvTile;
   const int64_t stride = value ? a.stride[1] : a.stride[0];
   const T *src = static_cast<const T *>(value ? a.src[1] : a.src[0]) + (int64_t)(u.row - first) * stride + head * (NB * 32);
+  float x[NB][2][8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int token = g + 8 * h;
+      if (token >= first && token < end) load_n<T, 8, VEC>(src + token * stride + b * 32 + t * 8, x[b][h]);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[b][h][i] = 0.0f;
+    }
   uint32_t w[NB][2];
-  if (!value) {
-    float x[NB][2][8];
+  uint8_t *const codes = rec + (value ? kv_value_codes(NB) : 0), *const scales = rec + (value ? kv_value_scales(NB) : kv_key_scales(NB));
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int token = g + 8 * h;
-        if (token >= first && token < end) load_n<T, 8, VEC>(src + token * stride + b * 32 + t * 8, x[b][h]);
-        else
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[b][h][i] = 0.0f;
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int token = g + 8 * h;
+      __half d;
+      w[b][h] = kv_quantise(x[b][h], t, &d);
+      if (t == 0 && token >= first && token < end) *reinterpret_cast<__half *>(scales + kv_scale(NB, b, token)) = d;
+    }
+  if (value) {
+    // this lane's word: dims 4 g on of tokens 2 t and 2 t + 1, from the lanes of those with dims 8 (g / 2) on
+    const int from = 8 * t + (g >> 1);
+    const uint32_t halves = g & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int token = g + 8 * h;
-        __half d;
-        w[b][h] = kv_quantise<8, 1>(x[b][h], t, &d);
-        if (token < first || token >= end) continue;
-        if (t == 0) *reinterpret_cast<__half *>(rec + kv_key_scales(NB) + kv_scale(NB, b, token)) = d;
-        if (!all) *reinterpret_cast<uint32_t *>(rec + kv_word(NB, b, lane, h)) = w[b][h];
+        const uint32_t even = __shfl_sync(0xffffffffu, w[b][h], from), odd = __shfl_sync(0xffffffffu, w[b][h], from + 4);
+        w[b][h] = __byte_perm(even, odd, halves);
       }
-  } else {
-    float x[NB][4][4];
+  }
+  if (all) {
 #pragma unroll
-    for (int y = 0; y < 4; ++y)
+    for (int b = 0; b + 1 < NB; b += 2)
+      *reinterpret_cast<uint4 *>(codes + kv_word(NB, b, lane, 0)) = make_uint4(w[b][0], w[b][1], w[b + 1][0], w[b + 1][1]);
+    if constexpr (NB % 2 == 1)
+      *reinterpret_cast<uint2 *>(codes + kv_word(NB, NB - 1, lane, 0)) = make_uint2(w[NB - 1][0], w[NB - 1][1]);
+    return;
+  }
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int token = 2 * t + (y & 1) + 8 * (y >> 1);
-        if (token >= first && token < end) load_n<T, 4, VEC>(src + token * stride + b * 32 + g * 4, x[b][y]);
-        else
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[b][y][i] = 0.0f;
-      }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      w[b][0] = w[b][1] = 0;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int token = 2 * t + (y & 1) + 8 * (y >> 1);
-        __half d;
-        const uint32_t codes = kv_quantise<4, 4>(x[b][y], g, &d);
-        w[b][y >> 1] |= codes << (16 * (y & 1));
-        if (token < first || token >= end) continue;
-        if (g == 0) *reinterpret_cast<__half *>(rec + kv_value_scales(NB) + kv_scale(NB, b, token)) = d;
-        if (!all)
-          *reinterpret_cast<uint16_t *>(rec + kv_value_codes(NB) + kv_word(NB, b, lane, y >> 1) + 2 * (y & 1)) = (uint16_t)codes;
+    for (int h = 0; h < 2; ++h) {
+      uint8_t *to = codes + kv_word(NB, b, lane, h);
+      auto is_new = [&](int token) { return token >= first && token < end; };
+      if (!value) {
+        if (is_new(g + 8 * h)) *reinterpret_cast<uint32_t *>(to) = w[b][h];
+      } else {
+        if (is_new(2 * t + 8 * h)) *reinterpret_cast<uint16_t *>(to) = (uint16_t)w[b][h];
+        if (is_new(2 * t + 1 + 8 * h)) *reinterpret_cast<uint16_t *>(to + 2) = (uint16_t)(w[b][h] >> 16);
       }
     }
-  }
-  if (!all) return;
-  uint8_t *to = rec + (value ? kv_value_codes(NB) : 0);
-#pragma unroll
-  for (int b = 0; b + 1 < NB; b += 2)
-    *reinterpret_cast<uint4 *>(to + kv_word(NB, b, lane, 0)) = make_uint4(w[b][0], w[b][1], w[b + 1][0], w[b + 1][1]);
-  if constexpr (NB % 2 == 1)
-    *reinterpret_cast<uint2 *>(to + kv_word(NB, NB - 1, lane, 0)) = make_uint2(w[NB - 1][0], w[NB - 1][1]);
 }
 
 template <typename T, int NB, bool VEC>
@@ -320,10 +333,10 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_read(const KvMove a) {
     }
 }
 
-// 16-byte accesses need rows that start on 16 bytes (a head's share is a
-// multiple of 64 bytes in every type).
+// Accesses of eight elements need rows that start on as many bytes (a head's
+// share is a multiple of 64 bytes in every type).
 bool vectors(const void *p, int64_t stride, int size) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * size) % 16 == 0;
+  return reinterpret_cast<uintptr_t>(p) % (8 * size) == 0 && stride % 8 == 0;
 }
 
 template <typename T, int NB>
