@@ -16,9 +16,9 @@ namespace {
 constexpr int kKvThreads = 256, kKvWarps = kKvThreads / 32;
 
 // A warp's work: the new rows of a sequence that fall into one 16-token tile,
-// for one head, keys or values.  Tiles are numbered so that a binary search
-// finds them: sequence b has the slots from offsets[b] / 16 + 2 b on, which are
-// as many as its rows can need wherever they start (n / 16 + 2).
+// for one head, keys or values.  Tiles are numbered so that a search finds
+// them: sequence b has the slots from offsets[b] / 16 + 2 b on, which are as
+// many as its rows can need wherever they start (n / 16 + 2).
 struct KvUnit {
   int seq, tile, lo, hi;  // tokens [lo, hi) of the tile are new
   int row;                // of token lo
@@ -33,11 +33,16 @@ __device__ __forceinline__ bool kv_unit(const KvRows &r, int64_t slot, KvUnit *u
     u->seq = (int)slot;
     len = r.lengths[slot], start = (int)slot, n = 1, first = 0;
   } else {
-    int64_t lo = 0, hi = r.sequences - 1;  // the last sequence whose slots start at or before `slot`
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (r.offsets[mid] / kKvTile + 2 * mid <= slot) lo = mid;
-      else hi = mid - 1;
+    // the last sequence whose slots start at or before `slot`: 32 of them are looked at at once
+    int64_t lo = 0;
+    for (int64_t left = r.sequences; left > 1;) {
+      const int64_t step = (left + 31) / 32, at = lo + (threadIdx.x & 31) * step;
+      const bool before = at < lo + left && r.offsets[at] / kKvTile + 2 * at <= slot;
+      const int hits = __popc(__ballot_sync(0xffffffffu, before));
+      if (hits == 0) return false;
+      const int64_t past = (hits - 1) * step;
+      lo += past;
+      left = left - past < step ? left - past : step;
     }
     u->seq = (int)lo;
     len = r.lengths[lo], start = r.offsets[lo];
