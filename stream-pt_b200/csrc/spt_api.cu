@@ -3457,6 +3457,7 @@ struct spt_kv_cache {
 struct spt_beam {
   spt_context *ctx = nullptr;
   spt_beam_config cfg{};
+  int chunks = 1;
   DevBuf work;
   DevBuf hlogits, hsmall;   // host calls' staging
 };
@@ -3478,6 +3479,8 @@ spt_status kv_config(spt_context *ctx, const spt_kv_config *c, int64_t *layer_by
                 (long long)c->page_tokens);
   if (c->pages > INT32_MAX || c->kv_heads > 4096 || c->layers > 65536)
     return fail(ctx, SPT_ERR_UNSUPPORTED, "KV cache dimensions exceed this build's limits");
+  if (c->layers * c->kv_heads * (c->page_tokens / kKvTile) * kv_tile_bytes((int)(c->head_dim / 32)) > (int64_t)16 * INT32_MAX)
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "a page of the KV cache is larger than 32 GiB over its layers");
   int64_t bytes = 0;
   if (!product({c->pages, c->kv_heads, c->page_tokens / kKvTile, kv_tile_bytes((int)(c->head_dim / 32))}, &bytes) ||
       !product({bytes, c->layers}, nullptr))
@@ -3880,8 +3883,8 @@ spt_status spt_beam_create(spt_context *ctx, const spt_beam_config *cfg, spt_bea
   if (!b) return fail(ctx, SPT_ERR_CUDA, "beam search: out of host memory");
   b->ctx = ctx;
   b->cfg = *cfg;
-  const cudaError_t e =
-      b->work.ensure(beam_workspace_bytes(cfg->batch, cfg->beams, cfg->vocab, (int)cfg->keep, ctx->sm_count));
+  b->chunks = beam_chunks(cfg->batch * cfg->beams, cfg->vocab, ctx->sm_count);
+  const cudaError_t e = b->work.ensure(beam_workspace_bytes(cfg->batch * cfg->beams, b->chunks, (int)cfg->keep));
   if (e != cudaSuccess) {
     cudaGetLastError();
     spt_beam_destroy(b);
@@ -3930,7 +3933,7 @@ spt_status spt_beam_select_device(spt_context *ctx, spt_beam *b, int32_t type, c
   a.out_parents = out_parents;
   a.out_tokens = out_tokens;
   a.work = b->work.p;
-  a.sm_count = ctx->sm_count;
+  a.chunks = b->chunks;
   SPT_CUDA(ctx, launch_beam_select(a, ctx->stream));
   ctx->kernels_last = 2;
   return SPT_OK;

@@ -284,6 +284,22 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_append(const KvMove a) {
     }
 }
 
+// (n - 8) d of the code n in nibble P (2 to 4) of a word, in two instructions:
+// the nibble in the mantissa of 2^E, E = 23 - 4 P, makes the float 2^E + n, and
+// (2^E + n) d - (2^E + 8) d is exact, as (2^E + 8) d has 23 bits at most.
+struct KvScale {
+  float d, off[3];
+  __device__ __forceinline__ explicit KvScale(float scale) : d(scale) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) off[i] = -((float)(1 << (15 - 4 * i)) + 8.0f) * scale;
+  }
+  template <int P>
+  __device__ __forceinline__ float times(uint32_t word) const {
+    return __fmaf_rn(__uint_as_float((word & 15u << (4 * P)) | (uint32_t)(127 + 23 - 4 * P) << 23), d, off[P - 2]);
+  }
+};
+
+// Bound by memory, as the records are read once and the rows written once.
 template <typename T, int NB, bool VEC>
 __global__ void __launch_bounds__(kKvThreads) k_kv_read(const KvMove a) {
   pdl_wait();
@@ -318,20 +334,19 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_read(const KvMove a) {
       if (!value) {
         const int token = g + 8 * h;
         if (token < first || token >= end) continue;
-        const float d = scale_of(b, h, g & 1);
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)((int)(word >> (4 * i) & 15u) - 8) * d;
+        const KvScale d(scale_of(b, h, g & 1));
+        const uint32_t up = word << 8, down = word >> 12;
+        const float x[8] = {d.times<2>(up),   d.times<3>(up),   d.times<2>(word), d.times<3>(word),
+                            d.times<4>(word), d.times<2>(down), d.times<3>(down), d.times<4>(down)};
         store_n<T, 8, VEC>(dst + token * stride + b * 32 + t * 8, x);
       } else {
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) {
           const int token = 2 * t + odd + 8 * h;
           if (token < first || token >= end) continue;
-          const float d = scale_of(b, h, odd);
-          float x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = (float)((int)(word >> (16 * odd + 4 * i) & 15u) - 8) * d;
+          const KvScale d(scale_of(b, h, odd));
+          const uint32_t low = odd ? word >> 8 : word << 8, high = odd ? word >> 16 : word;
+          const float x[4] = {d.times<2>(low), d.times<3>(low), d.times<2>(high), d.times<3>(high)};
           store_n<T, 4, VEC>(dst + token * stride + b * 32 + g * 4, x);
         }
       }
@@ -394,7 +409,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_reorder(uint8_t *pool, int64_
   const int64_t from = valid ? b * a.beams + parent : 0;
   int64_t len = valid ? a.lengths[from] : 0;
   len = len < 0 ? 0 : len > a.max_pages * c.page_tokens ? a.max_pages * c.page_tokens : len;
-  const int64_t full = len / c.page_tokens;
+  const int64_t full = (uint32_t)len / (uint32_t)c.page_tokens;  // (len is an int32)
   const int rest = (int)(len - full * c.page_tokens);
   bool later = false;
   for (int64_t i = 0; i < j; ++i) later |= parents[i] == parent;
@@ -412,9 +427,9 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_reorder(uint8_t *pool, int64_
   }
   if (!copy || old == own) return;
   const int per_head = (rest + kKvTile - 1) / kKvTile * (kv_tile_bytes(c.nb) / 16);  // 16-byte words
-  const int64_t words = layers * c.kv_heads * per_head;
-  for (int64_t w = (int64_t)blockIdx.y * kKvThreads + threadIdx.x; w < words; w += (int64_t)gridDim.y * kKvThreads) {
-    const int64_t lh = w / per_head, layer = lh / c.kv_heads;
+  const uint32_t words = (uint32_t)layers * c.kv_heads * per_head;
+  for (uint32_t w = blockIdx.y * kKvThreads + threadIdx.x; w < words; w += gridDim.y * kKvThreads) {
+    const uint32_t lh = w / per_head, layer = lh / c.kv_heads;
     const int head = (int)(lh - layer * c.kv_heads), at = (int)(w - lh * per_head);
     uint8_t *base = pool + layer * layer_bytes + (int64_t)at * 16;
     *reinterpret_cast<uint4 *>(base + kv_tile_offset(c, own, head, 0)) =

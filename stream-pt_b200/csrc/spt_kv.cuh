@@ -145,9 +145,10 @@ struct BeamArgs {
   float *out_scores = nullptr;
   int32_t *out_parents = nullptr, *out_tokens = nullptr;
   void *work = nullptr;          // beam_workspace_bytes()
-  int sm_count = 148;
+  int chunks = 1;                // beam_chunks()
 };
-size_t beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int keep, int sm_count);
+int beam_chunks(int64_t rows, int64_t vocab, int sm_count);  // CTAs a row's logits are cut into
+size_t beam_workspace_bytes(int64_t rows, int chunks, int keep);
 cudaError_t launch_beam_select(const BeamArgs &a, cudaStream_t stream);
 
 }  // namespace spt

@@ -96,6 +96,38 @@ def test_strided_rows(ctx):
         check(ctx, wide.half()[:, :, :9001], [[0.0, -1.0, -2.0]], 6)
 
 
+@pytest.mark.parametrize("pattern", ["rising", "falling", "ties", "few", "lowest", "masked", "late", "nan", "large", "inf"])
+@pytest.mark.parametrize("type,keep,vocab", [("f32", 64, 30001), ("bf16", 7, 24576), ("f16", 16, 29999)])
+def test_long_rows(ctx, pattern, type, keep, vocab):
+    """Many rows of several pieces each: candidates that outrun the list, masks over whole pieces."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(keep)
+    x = torch.randn(6, 64, vocab, generator=gen, device="cuda") * 2
+    inf = float("inf")
+    if pattern in ("rising", "falling"):
+        x = x.sort(-1, descending=pattern == "falling").values
+    elif pattern == "ties":
+        x = torch.zeros_like(x)
+    elif pattern == "few":
+        x = x.round()
+    elif pattern == "lowest":  # rows of nothing but the type's lowest value, and rows that end with it
+        x[:, ::2] = x[:, 1::2, 9000:] = torch.finfo(torch_type(type)).min
+    elif pattern == "masked":
+        x[:, :, 100:20000] = -inf
+        x[:, 5] = -inf
+    elif pattern == "late":  # everything that counts in the last piece
+        x[:, :, :-70] = -inf
+    elif pattern == "nan":
+        x[:, :, 1::2] = float("nan")
+        x[:, 3, :20000] = float("nan")
+    elif pattern == "large":
+        x = x * (1e30 if type != "f16" else 1e4)
+    elif pattern == "inf":
+        x[:, ::3, 20000] = inf
+    scores = np.random.default_rng(keep).normal(size=(6, 64)) - 4
+    check(ctx, x.to(torch_type(type)), scores, keep)
+
+
 def test_host_call_and_refusals(ctx):
     rng = np.random.default_rng(1)
     plan = ctx.beam(2, 3, 500, 6)
