@@ -3509,6 +3509,10 @@ spt_status kv_call(spt_context *ctx, const spt_kv_cache *cache, int64_t layer, c
   if (r->sequences < 0 || r->tokens < 0 || r->max_pages < 0 || r->sequences > INT32_MAX || r->tokens > INT32_MAX ||
       r->max_pages > INT32_MAX)
     return fail(ctx, SPT_ERR_DIMENSIONS, "invalid KV row counts");
+  // (a warp of the cache's kernels per 16-token tile and head, at most two tiles a sequence more than its rows fill)
+  if ((r->tokens / kKvTile + 2 * r->sequences + 1) * cache->cfg.kv_heads > INT32_MAX ||
+      r->sequences * r->max_pages > ((int64_t)1 << 40))
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "KV row counts exceed this build's limits");
   if (r->sequences > 0 && (!r->lengths || (!r->table && r->max_pages > 0)))
     return fail(ctx, SPT_ERR_NULL_ARG, "nil page table or lengths");
   if (!aligned(r->table, 4) || !aligned(r->lengths, 4) || !aligned(r->offsets, 4))
@@ -3534,13 +3538,14 @@ spt_status row_array(spt_context *ctx, const void *p, int32_t type, int64_t widt
   if (*stride == 0) *stride = width;
   if (*stride < width) return fail(ctx, SPT_ERR_DIMENSIONS, "row stride %lld below the row's %lld elements",
                                    (long long)*stride, (long long)width);
-  if (*stride > ((int64_t)1 << 40)) return fail(ctx, SPT_ERR_DIMENSIONS, "row stride %lld", (long long)*stride);
-  (void)tokens;
+  if (*stride > ((int64_t)1 << 58) / (tokens > 0 ? tokens : 1))
+    return fail(ctx, SPT_ERR_DIMENSIONS, "row stride %lld", (long long)*stride);
   if (!aligned(p, size)) return fail(ctx, SPT_ERR_DIMENSIONS, "rows not aligned to their type");
   return SPT_OK;
 }
 
-spt_status attention_config(spt_context *ctx, const spt_kv_cache *cache, const spt_attention_config *cfg) {
+spt_status attention_config(spt_context *ctx, const spt_kv_cache *cache, const spt_attention_config *cfg,
+                            int64_t tokens) {
   if (!cfg) return fail(ctx, SPT_ERR_NULL_ARG, "nil attention configuration");
   if (cfg->heads <= 0 || cfg->heads % cache->cfg.kv_heads != 0 || cfg->heads > 65536)
     return fail(ctx, SPT_ERR_DIMENSIONS, "%lld query heads on %lld key heads", (long long)cfg->heads,
@@ -3549,6 +3554,9 @@ spt_status attention_config(spt_context *ctx, const spt_kv_cache *cache, const s
   if (!(cfg->scale > 0.0f) || !std::isfinite(cfg->scale))
     return fail(ctx, SPT_ERR_DIMENSIONS, "attention scale %g", (double)cfg->scale);
   if (!aligned(cfg->sinks, 4)) return fail(ctx, SPT_ERR_DIMENSIONS, "sinks not aligned to 4 bytes");
+  if (tokens > INT32_MAX / (cfg->heads / cache->cfg.kv_heads))
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "%lld query rows of %lld heads exceed this build's limits", (long long)tokens,
+                (long long)cfg->heads);
   return SPT_OK;
 }
 
@@ -3623,7 +3631,7 @@ spt_status reorder_args(spt_context *ctx, const spt_kv_cache *cache, int64_t bat
   if (cache->ctx != ctx) return fail(ctx, SPT_ERR_DIMENSIONS, "KV cache belongs to another context");
   int64_t n = 0;
   if (batch <= 0 || beams <= 0 || max_pages <= 0 || parents_stride < beams || !product({batch, beams}, &n) ||
-      n > INT32_MAX || max_pages > INT32_MAX || parents_stride > INT32_MAX)
+      n > INT32_MAX || max_pages > INT32_MAX || parents_stride > INT32_MAX || n * max_pages > ((int64_t)1 << 40))
     return fail(ctx, SPT_ERR_DIMENSIONS, "invalid beam reorder dimensions");
   if (beams > kBeamMaxBeams) return fail(ctx, SPT_ERR_UNSUPPORTED, "%lld beams", (long long)beams);
   if (!parents || !table || !lengths || !spare || !table_out || !lengths_out)
@@ -3713,7 +3721,7 @@ spt_status spt_kv_append_device(spt_context *ctx, spt_kv_cache *cache, int64_t l
   if (rows->tokens > 0 && (!k || !v)) return fail(ctx, SPT_ERR_NULL_ARG, "nil key or value rows");
   if ((st = require_device(ctx))) return st;
   SPT_CUDA(ctx, launch_kv_append(kv_layer(cache, layer), kv_rows(rows), type, k, k_stride, v, v_stride, ctx->stream));
-  ctx->kernels_last = 1;
+  ctx->kernels_last = rows->tokens > 0 && rows->sequences > 0;
   return SPT_OK;
 }
 
@@ -3724,10 +3732,18 @@ spt_status spt_kv_read_device(spt_context *ctx, spt_kv_cache *cache, int64_t lay
   const int64_t width = cache->cfg.kv_heads * cache->cfg.head_dim;
   if ((st = row_array(ctx, k, type, width, rows->tokens, &k_stride))) return st;
   if ((st = row_array(ctx, v, type, width, rows->tokens, &v_stride))) return st;
+  const int size = type_size(type);
+  if (k && v && rows->tokens > 0 && ranges_overlap(k, ((rows->tokens - 1) * k_stride + width) * size, v,
+                                                   ((rows->tokens - 1) * v_stride + width) * size)) {
+    // (rows of both in turn in one buffer are fine)
+    const int64_t apart = (int64_t)((uintptr_t)v - (uintptr_t)k) / size, at = (apart % k_stride + k_stride) % k_stride;
+    if (k_stride != v_stride || at < width || at > k_stride - width)
+      return fail(ctx, SPT_ERR_OVERLAP, "key and value rows must not overlap");
+  }
   if ((st = require_device(ctx))) return st;
   if (!k && !v) return SPT_OK;
   SPT_CUDA(ctx, launch_kv_read(kv_layer(cache, layer), kv_rows(rows), type, k, k_stride, v, v_stride, ctx->stream));
-  ctx->kernels_last = 1;
+  ctx->kernels_last = rows->tokens > 0 && rows->sequences > 0;
   return SPT_OK;
 }
 
@@ -3736,7 +3752,7 @@ spt_status spt_attention_device(spt_context *ctx, spt_kv_cache *cache, int64_t l
                                 void *out, int64_t out_stride) {
   spt_status st = kv_call(ctx, cache, layer, rows);
   if (st) return st;
-  if ((st = attention_config(ctx, cache, cfg))) return st;
+  if ((st = attention_config(ctx, cache, cfg, rows->tokens))) return st;
   const int64_t width = cfg->heads * cache->cfg.head_dim;
   if ((st = row_array(ctx, q, type, width, rows->tokens, &q_stride))) return st;
   if ((st = row_array(ctx, out, type, width, rows->tokens, &out_stride))) return st;
@@ -3768,7 +3784,7 @@ spt_status spt_attention_device(spt_context *ctx, spt_kv_cache *cache, int64_t l
   a.fault_tile = ctx->opt_fault_stage;
   a.sm_count = ctx->sm_count;
   SPT_CUDA(ctx, launch_attention(a, ctx->stream));
-  ctx->kernels_last = 1;
+  ctx->kernels_last = rows->tokens > 0 && rows->sequences > 0;
   return SPT_OK;
 }
 
@@ -3834,7 +3850,7 @@ spt_status spt_attention(spt_context *ctx, spt_kv_cache *cache, int64_t layer, c
                          int64_t out_len, const volatile int32_t *cancel) {
   spt_status st = kv_call(ctx, cache, layer, rows);
   if (st) return st;
-  if ((st = attention_config(ctx, cache, cfg))) return st;
+  if ((st = attention_config(ctx, cache, cfg, rows->tokens))) return st;
   const int64_t n = rows->tokens * cfg->heads * cache->cfg.head_dim;
   if (q_len != n || out_len != n)
     return fail(ctx, SPT_ERR_DIMENSIONS, "expected %lld query and output elements, got %lld and %lld", (long long)n,
@@ -3917,6 +3933,19 @@ spt_status spt_beam_select_device(spt_context *ctx, spt_beam *b, int32_t type, c
   if (finished && (end_token < 0 || end_token >= b->cfg.vocab))
     return fail(ctx, SPT_ERR_DIMENSIONS, "end token %lld outside the vocabulary of %lld", (long long)end_token,
                 (long long)b->cfg.vocab);
+  const int64_t rows = b->cfg.batch * b->cfg.beams, kept = b->cfg.batch * b->cfg.keep * 4;
+  const struct { const void *p; int64_t n; } in[] = {
+      {logits, ((rows - 1) * row_stride + b->cfg.vocab) * type_size(type)}, {scores, rows * 4},
+      {finished, finished ? rows : 0}};
+  const void *out[] = {out_scores, out_parents, out_tokens};
+  for (int i = 0; i < 3; ++i) {
+    for (const auto &x : in)
+      if (ranges_overlap(x.p, x.n, out[i], kept))
+        return fail(ctx, SPT_ERR_OVERLAP, "beam search inputs and outputs must not overlap");
+    for (int j = 0; j < i; ++j)
+      if (ranges_overlap(out[i], kept, out[j], kept))
+        return fail(ctx, SPT_ERR_OVERLAP, "beam search outputs must not overlap");
+  }
   if ((st = require_device(ctx))) return st;
   BeamArgs a;
   a.logits = logits;

@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
       // O^T += V^T P^T.  With two terms the step's products are summed from
       // zero and added in f32: the tensor cores' own additions lose bits of a
       // long sum.
-      float oc[NT][NB][2][4];
+      [[maybe_unused]] float oc[NT][NB][2][4];
       if constexpr (TERMS == 2) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
           const uint32_t a0[4] = {e0[0], e0[1], e1[0], e1[1]}, a1[4] = {e0[2], e0[3], e1[2], e1[3]};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint32_t hi[2], lo[2];
+            [[maybe_unused]] uint32_t hi[2], lo[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float2 p = __fmul2_rn(s[i][nt][h], __half22float2(half2_of(h ? vd.y : vd.x)));
@@ -545,7 +545,14 @@ cudaError_t launch_attention(const AttnArgs &args, cudaStream_t stream) {
   const int size = a.type == kKvF32 ? 4 : 2;
   a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * size)) & 15) == 0;
   a.out_vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * size)) & 15) == 0;
-  if (a.r.offsets && a.r.tokens * a.group > 32 * a.r.sequences) return launch_attention_mma(a, stream);
+  // Query rows a sequence and key head, on average, from which the tensor cores'
+  // 128-row tiles pay although most of a tile may be empty.  16 sequences of
+  // 8,000 keys, 8 key heads, this kernel against those tiles, us: dim 64, f32,
+  // 32 rows 93 : 208, 64 rows 175 : 202, 128 rows 334 : 188; bf16 64 rows 122 :
+  // 198, 128 rows 226 : 183; dim 128, f32, 32 rows 190 : 236, 64 rows 362 : 237;
+  // bf16 64 rows 234 : 231, 128 rows 446 : 211.
+  const int64_t few = a.type == kKvF32 && a.c.nb > 2 ? 32 : 64;
+  if (a.r.offsets && a.r.tokens * a.group > few * a.r.sequences) return launch_attention_mma(a, stream);
   switch (a.type) {
     case kKvF32: return launch_dims<float>(a, stream);
     case kKvF16: return launch_dims<__half>(a, stream);

@@ -155,6 +155,10 @@ def test_host_call_and_refusals(ctx):
     refused(dim, lambda: plan.select_device(p, p + 1, p, p, p))
     refused(dim, lambda: plan.select_device(p, p, p, p, p, finished_ptr=p, end_token=-1))
     refused(spt.ERR_NULL_ARG, lambda: plan.select_device(0, p, p, p, p))
+    o = [torch.zeros(64, device="cuda").data_ptr() for _ in range(3)]
+    refused(spt.ERR_OVERLAP, lambda: plan.select_device(p, p, p, o[1], o[2]))           # scores in place
+    refused(spt.ERR_OVERLAP, lambda: plan.select_device(p, p, o[0], p + 4 * 2999, o[2]))  # the last logit
+    refused(spt.ERR_OVERLAP, lambda: plan.select_device(p, p, o[0], o[1], o[1] + 44))
     refused(spt.ERR_UNSUPPORTED, lambda: plan.select_device(p, p, p, p, p, type=8))
     plan.close()
 

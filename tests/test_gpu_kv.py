@@ -154,6 +154,43 @@ def test_host_calls(ctx):
     cache.close()
 
 
+def test_limits_and_overlaps(ctx):
+    """Counts beyond what a launch numbers, strides beyond 64 bits, outputs on top of one another; a
+    buffer whose rows are keys and values in turn is none of these."""
+    import torch
+    cache = ctx.kv_cache(kv_heads=2, head_dim=64, page_tokens=16, pages=3)
+    table, lengths = np.array([[0, 1]], np.int32), np.array([17], np.int32)
+    rng = np.random.default_rng(3)
+    x = rng.normal(size=(17, 2, 64)).astype(np.float32)
+    cache.append(spt.KvBatch(1, 17, 2, table, lengths, [0, 17]), x, -x)
+    dev = Device(table, [17], [17])
+    p = torch.zeros(17, 256, device="cuda")
+
+    def refused(status, call):
+        with pytest.raises(spt.SptError) as e:
+            call()
+        assert e.value.status == status, e.value
+
+    d, n = p.data_ptr(), 2 ** 31 - 1
+    big = lambda **c: spt.KvBatch(**{**dict(sequences=1, tokens=17, max_pages=2, table=d, lengths=d, offsets=d), **c})  # noqa: E731
+    for call in (cache.append_device, cache.read_device):
+        refused(spt.ERR_UNSUPPORTED, lambda: call(big(sequences=n), d, d))
+        refused(spt.ERR_UNSUPPORTED, lambda: call(big(sequences=2 ** 21, max_pages=2 ** 20), d, d))
+        refused(spt.ERR_DIMENSIONS, lambda: call(big(), d, d, k_stride=2 ** 60))
+        refused(spt.ERR_DIMENSIONS, lambda: call(big(tokens=n), d, d, v_stride=2 ** 40))
+    refused(spt.ERR_UNSUPPORTED, lambda: cache.attention_device(big(tokens=n), d, d, heads=4))
+    refused(spt.ERR_OVERLAP, lambda: cache.read_device(dev.batch, d, d))
+    refused(spt.ERR_OVERLAP, lambda: cache.read_device(dev.batch, d, d + 4 * 64, k_stride=256, v_stride=256))
+    refused(spt.ERR_OVERLAP, lambda: cache.read_device(dev.batch, d, d + 4 * 256, k_stride=128, v_stride=256))
+    refused(spt.ERR_UNSUPPORTED, lambda: ctx.validate_kv(kv_heads=64, head_dim=128, page_tokens=65536, pages=2, layers=128))
+    torch.cuda.synchronize()
+    cache.read_device(dev.batch, d, d + 4 * 128, k_stride=256, v_stride=256)
+    ctx.sync()
+    got = p.cpu().numpy().reshape(17, 2, 2, 64)
+    assert np.array_equal(got[:, 0], held(x).astype(np.float32)) and np.array_equal(got[:, 1], held(-x).astype(np.float32))
+    cache.close()
+
+
 def test_calls_refused(ctx):
     import torch
     cache = ctx.kv_cache(kv_heads=2, head_dim=64, page_tokens=16, pages=3)
