@@ -26,41 +26,42 @@ struct KvUnit {
 inline int64_t kv_slots(const KvRows &r) {
   return r.offsets ? r.tokens / kKvTile + 2 * r.sequences + 1 : r.sequences < r.tokens ? r.sequences : r.tokens;
 }
-__device__ __forceinline__ bool kv_unit(const KvRows &r, int64_t slot, KvUnit *u) {
-  int len, start, n, first;  // first: the slot of the sequence's first tile, less `slot`
+// (slots fit 31 bits: the callers' row counts are checked for it)
+__device__ __forceinline__ bool kv_unit(const KvRows &r, uint32_t slot, KvUnit *u) {
+  int len, start, n;
+  uint32_t first;  // the slot, counted from the sequence's first
   if (!r.offsets) {
     if (slot >= r.sequences || slot >= r.tokens) return false;
     u->seq = (int)slot;
     len = r.lengths[slot], start = (int)slot, n = 1, first = 0;
   } else {
     // the last sequence whose slots start at or before `slot`: 32 of them are looked at at once
-    int64_t lo = 0;
-    for (int64_t left = r.sequences; left > 1;) {
-      const int64_t step = (left + 31) / 32, at = lo + (threadIdx.x & 31) * step;
-      const bool before = at < lo + left && r.offsets[at] / kKvTile + 2 * at <= slot;
+    uint32_t lo = 0;
+    for (uint32_t left = (uint32_t)r.sequences; left > 1;) {
+      const uint32_t step = (left + 31) >> 5, at = lo + (threadIdx.x & 31) * step;
+      const bool before = at < lo + left && (uint32_t)(r.offsets[at] >> 4) + 2 * at <= slot;
       const int hits = __popc(__ballot_sync(0xffffffffu, before));
       if (hits == 0) return false;
-      const int64_t past = (hits - 1) * step;
+      const uint32_t past = (uint32_t)(hits - 1) * step;
       lo += past;
-      left = left - past < step ? left - past : step;
+      left = min(left - past, step);
     }
     u->seq = (int)lo;
     len = r.lengths[lo], start = r.offsets[lo];
     const int end = r.offsets[lo + 1];
     if (start < 0 || end > r.tokens || end <= start) return false;
     n = end - start;
-    const int64_t past = slot - (start / kKvTile + 2 * lo);
-    if (past < 0 || past > n / kKvTile + 1) return false;
-    first = (int)past;
+    first = slot - ((uint32_t)start / kKvTile + 2 * lo);
+    if (first > (uint32_t)n / kKvTile + 1) return false;  // (before the first slot: beyond any)
   }
   const int64_t pos0 = (int64_t)len - n;  // (rows before position 0 have no place)
-  const int p0 = pos0 > 0 ? (int)pos0 : 0;
-  u->tile = p0 / kKvTile + first;
-  const int64_t from = (int64_t)u->tile * kKvTile;
-  u->lo = (int)(from > p0 ? from : p0);
-  u->hi = (int)(from + kKvTile < len ? from + kKvTile : len);
-  u->row = start + (int)(u->lo - pos0);
-  return u->lo < u->hi;
+  const uint32_t p0 = pos0 > 0 ? (uint32_t)pos0 : 0, tile = p0 / kKvTile + first, from = tile * kKvTile;
+  const int64_t lo = from > p0 ? from : p0, hi = len < (int64_t)from + kKvTile ? len : (int64_t)from + kKvTile;
+  u->tile = (int)tile;
+  u->lo = (int)lo;
+  u->hi = (int)hi;
+  u->row = start + (int)(lo - pos0);
+  return lo < hi;
 }
 
 template <typename T>
@@ -198,10 +199,10 @@ struct KvMove {
 __device__ __forceinline__ uint8_t *kv_record(const KvMove &a, KvUnit *u, int *head) {
   const int64_t id = (int64_t)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
   if (id >= a.units) return nullptr;
-  const int64_t slot = (uint32_t)id / (uint32_t)a.c.kv_heads;
-  *head = (int)(id - slot * a.c.kv_heads);
+  const uint32_t slot = (uint32_t)id / (uint32_t)a.c.kv_heads;
+  *head = (int)((uint32_t)id - slot * a.c.kv_heads);
   if (!kv_unit(a.r, slot, u)) return nullptr;
-  const int tiles = a.c.page_tokens / kKvTile, entry = u->tile / tiles;
+  const int tiles = a.c.page_tokens / kKvTile, entry = (int)((uint32_t)u->tile / (uint32_t)tiles);
   if (entry >= a.r.max_pages) return nullptr;
   const int64_t page = a.r.table[u->seq * a.r.max_pages + entry];
   if (page < 0 || page >= a.c.pages) return nullptr;
