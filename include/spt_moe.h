@@ -16,6 +16,11 @@
  *   spt_mul_q80                  MulQ80Into/Argmax forward/q80.go:22-148
  *   spt_mul_q40                  MulQ40Into        forward/q40.go:35-40
  *   spt_mul_q40_batch            MulQ40BatchInto   forward/q40.go:46-101
+ *   spt_kv_append, spt_attention the fp32 cache and the attention over it
+ *                                forward/attention.go:59-160 (here 4 bits a
+ *                                value, paged, for many sequences at once)
+ *   spt_beam_select, spt_kv_reorder
+ *                                none: beam search beside MulQ80Argmax
  *   spt_arena_create             ggufmap.WithExpertRanges + readExpertBias
  *                                (ggufmap/mmap_linux.go:391-555, forward/moe.go:72-92):
  *                                the streamed mmap window becomes an HBM arena
@@ -436,7 +441,7 @@ typedef struct spt_kv_config {
   int64_t layers;
   int64_t kv_heads;
   int64_t head_dim;    /* 32, 64, 96 or 128 */
-  int64_t page_tokens; /* a multiple of 16, at most 65536 */
+  int64_t page_tokens; /* a multiple of 16, at most 65536; a page at most 32 GiB over all layers */
   int64_t pages;       /* at most 2^31 - 1 */
 } spt_kv_config;
 typedef struct spt_kv_cache spt_kv_cache;
@@ -470,7 +475,8 @@ typedef struct spt_kv_rows {
  * place of the same page: pages that sequences share are for reading. */
 spt_status spt_kv_append_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
                                 int32_t type, const void *k, int64_t k_stride, const void *v, int64_t v_stride);
-/* The same rows as the cache holds them (k or v may be NULL). */
+/* The same rows as the cache holds them (k or v may be NULL; rows of both in
+ * turn in one buffer are fine, else they do not overlap). */
 spt_status spt_kv_read_device(spt_context *ctx, spt_kv_cache *cache, int64_t layer, const spt_kv_rows *rows,
                               int32_t type, void *k, int64_t k_stride, void *v, int64_t v_stride);
 
@@ -509,8 +515,8 @@ spt_status spt_attention(spt_context *ctx, spt_kv_cache *cache, int64_t layer, c
  * best first, equal scores in the order of beam and token.  A finished beam
  * (finished may be NULL) offers end_token alone, with its score unchanged.  A
  * NaN logit is no token, a score that is NaN or -inf (an unused beam's) no
- * candidate; places without one get score -inf, parent -1, token -1.  The
- * handle keeps the workspace of one call: its calls have to be serialised. */
+ * candidate; places without one get score -inf, parent -1, token -1.  Inputs
+ * and outputs do not overlap (SPT_ERR_OVERLAP).  The handle keeps the workspace of one call: its calls have to be serialised. */
 typedef struct spt_beam_config {
   int64_t batch;
   int64_t beams; /* at most 64; batch * beams at most 65535 */

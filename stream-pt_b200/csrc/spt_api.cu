@@ -3479,12 +3479,12 @@ spt_status kv_config(spt_context *ctx, const spt_kv_config *c, int64_t *layer_by
                 (long long)c->page_tokens);
   if (c->pages > INT32_MAX || c->kv_heads > 4096 || c->layers > 65536)
     return fail(ctx, SPT_ERR_UNSUPPORTED, "KV cache dimensions exceed this build's limits");
-  if (c->layers * c->kv_heads * (c->page_tokens / kKvTile) * kv_tile_bytes((int)(c->head_dim / 32)) > (int64_t)16 * INT32_MAX)
-    return fail(ctx, SPT_ERR_UNSUPPORTED, "a page of the KV cache is larger than 32 GiB over its layers");
   int64_t bytes = 0;
   if (!product({c->pages, c->kv_heads, c->page_tokens / kKvTile, kv_tile_bytes((int)(c->head_dim / 32))}, &bytes) ||
       !product({bytes, c->layers}, nullptr))
     return fail(ctx, SPT_ERR_DIMENSIONS, "KV cache size overflows");
+  if (c->layers * c->kv_heads * (c->page_tokens / kKvTile) * kv_tile_bytes((int)(c->head_dim / 32)) > (int64_t)16 * INT32_MAX)
+    return fail(ctx, SPT_ERR_UNSUPPORTED, "a page of the KV cache is larger than 32 GiB over its layers");
   if (layer_bytes) *layer_bytes = bytes;
   return SPT_OK;
 }

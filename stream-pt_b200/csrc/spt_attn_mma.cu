@@ -23,7 +23,12 @@
 //
 // Bound, for 256 rows x 64 keys at head_dim 64: 1,024 clocks of exponentials
 // (16 a clock on an SM), 1,584 of MMA for f32 rows (48 of 33 clocks) and 1,056
-// for 16-bit rows.
+// for 16-bit rows.  A tile takes 3,300 clocks (f32) or 3,000 (16 bits), those of
+// the softmax warps' own chain: 200 to wait, 350 to fetch S, 300 for its maximum,
+// 1,650 for the weights, 650 to add O, two warps a scheduler.  A prompt of 2,000
+// f32 rows (64 heads on 8 of 64 dims) takes 160 us, tensor cores 32% busy; f16
+// chunks of 12 sequences, 3,000 tokens each, 225 us.  Maxima of three instead of
+// two, or each MMA's S right behind its own O, changed neither by 1%.
 #include "spt_attn.cuh"
 
 namespace spt {

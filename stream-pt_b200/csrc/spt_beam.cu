@@ -152,7 +152,9 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) k_beam_chunk(const Be
   // keep distinct logits are at least the smallest of the maxima of as many groups of lanes
   int group = 32;
   while (kBeamThreads / group < a.keep) group >>= 1;
-  auto stage = [&](int piece) { return reinterpret_cast<uint4 *>(stages) + (piece - first) % kBeamStages * (kLoads * kBeamThreads) + tid; };
+  auto stage = [&](int piece) {
+    return reinterpret_cast<uint4 *>(stages) + (piece - first) % kBeamStages * (kLoads * kBeamThreads) + tid;
+  };
   // place in its piece of logit j of load i
   auto place = [&](int i, int j) { return (i * kBeamThreads + tid) * V + j; };
   auto fetch = [&](int piece) {
@@ -252,7 +254,8 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamCtas) k_beam_chunk(const Be
     }
     float part = ((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y)) * exp2f(-extra);
     if (!(part < INFINITY) || fabsf(shift) > 1e6f) {
-      // a NaN, which is left out (an infinite logit makes its row's sum one), or a shift whose product with L is too coarse
+      // a NaN, which is left out (an infinite logit makes its row's sum one), or a
+      // shift whose product with L is too coarse
       part = 0.0f;
 #pragma unroll 1
       for (int i = 0; i < kLoads; ++i)

@@ -209,7 +209,11 @@ __device__ __forceinline__ uint8_t *kv_record(const KvMove &a, KvUnit *u, int *h
   return a.c.base + kv_tile_offset(a.c, page, *head, (u->tile - entry * tiles) * kKvTile);
 }
 
-// Bound by memory: rows are read once and the records written once.  Lane 4 g +
+// Rows are read once and the records written once; bound by instructions on the
+// way, 29 for a value of each lane, and in small calls by latency (24 prompts,
+// 17,700 f32 tokens of 8 heads of 64 dims: 27 us under a profiler, 3.1 TB/s, at
+// 0.68 instructions a clock).  A tile is a warp's, as its record is what the attention reads
+// whole.  Lane 4 g +
 // t quantises dims 8 t on of each block of tokens g and g + 8; that is the
 // keys' layout, and for the values' two lanes' words are exchanged for their
 // halves.  A tile whose 16 tokens are all new leaves as 16-byte pieces; else
@@ -300,7 +304,8 @@ struct KvScale {
   }
 };
 
-// Bound by memory, as the records are read once and the rows written once.
+// The records are read once and the rows written once: 18 us under a profiler for
+// the tokens above, 4.6 TB/s, at 0.62 instructions a clock.
 template <typename T, int NB, bool VEC>
 __global__ void __launch_bounds__(kKvThreads) k_kv_read(const KvMove a) {
   pdl_wait();
@@ -398,7 +403,9 @@ cudaError_t launch_typed(KvMove a, int type, bool append, cudaStream_t stream) {
 // One CTA row per sequence (blockIdx.x) and share of the copy (blockIdx.y).
 // A child takes its parent's whole pages by number; the parent's partial last
 // page goes to its first child, every later child gets a copy of the tiles in
-// use, on every layer.
+// use, on every layer.  Bound by latency: a chain of table look-ups before a copy
+// of a few KB (128 beams, 4 layers: 9.4 us alone; a launch that copies nothing
+// takes about 4).
 __global__ void __launch_bounds__(kKvThreads) k_kv_reorder(uint8_t *pool, int64_t layers, int64_t layer_bytes,
                                                           const KvLayer c, const KvReorder a) {
   pdl_wait();
