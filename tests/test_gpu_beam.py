@@ -217,6 +217,56 @@ def test_reorder(ctx, lengths, parents):
     cache.close()
 
 
+def test_step_captured_and_replayed(ctx):
+    """Selection, reorder and the read-back in a graph: replayed on other logits it does what the calls do."""
+    import torch
+    page, heads, dim, beams, keep, vocab = 16, 2, 64, 3, 6, 20011
+    lengths = [21, 40, 5, 33, 16, 50]
+    table, spare, pages = random_table(np.random.default_rng(7), lengths, page, spare=6)
+    cache = ctx.kv_cache(kv_heads=heads, head_dim=dim, page_tokens=page, pages=pages)
+    plan = ctx.beam(2, beams, vocab, keep)
+    dev = Device(table, lengths, lengths)
+    data = torch.randn(sum(lengths), heads, dim, device="cuda")
+    torch.cuda.synchronize()
+    cache.append_device(dev.batch, data.data_ptr(), data.data_ptr())
+    x, scores = torch.empty(6, vocab, device="cuda"), torch.full((6,), -1.0, device="cuda")
+    sp = torch.tensor(spare[:6], dtype=torch.int32, device="cuda")
+
+    def outputs():
+        i32 = lambda *n: torch.full(n, 99, dtype=torch.int32, device="cuda")  # noqa: E731
+        return dict(scores=torch.empty(2, keep, device="cuda"), parents=i32(2, keep), tokens=i32(2, keep),
+                    table=i32(*dev.table.shape), lengths=i32(6), rows=torch.zeros(6, heads, dim, device="cuda"))
+
+    def step(o):
+        p = {k: v.data_ptr() for k, v in o.items()}
+        plan.select_device(x.data_ptr(), scores.data_ptr(), p["scores"], p["parents"], p["tokens"])
+        cache.reorder_device(2, beams, table.shape[1], p["parents"], keep, dev.table.data_ptr(), dev.lengths.data_ptr(),
+                             sp.data_ptr(), p["table"], p["lengths"], 0)
+        cache.read_device(spt.KvBatch(6, 6, table.shape[1], p["table"], p["lengths"]), p["rows"], 0)
+
+    eager, held_out, stream = outputs(), outputs(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step(held_out)
+        for seed in range(3):
+            x.copy_(torch.randn(6, vocab, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            step(eager)
+            ctx.sync()
+            for name in eager:
+                assert torch.equal(eager[name], held_out[name]), (seed, name)
+            assert int((eager["lengths"] > 0).sum()) == 6 and bool((eager["rows"] != 0).any())
+    finally:
+        ctx.set_stream(0)
+    plan.close()
+    cache.close()
+
+
 def test_reorder_host_and_refusals(ctx):
     cache = ctx.kv_cache(kv_heads=1, head_dim=32, page_tokens=16, pages=8)
     rng = np.random.default_rng(0)
