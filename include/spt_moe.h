@@ -487,8 +487,9 @@ spt_status spt_kv_read_device(spt_context *ctx, spt_kv_cache *cache, int64_t lay
  *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[head]))
  * without the sink term where sinks is NULL.  A row without keys is 0.  A row
  * of q with a NaN or an infinity gives NaNs and touches no other row.  The
- * sums are held in 32 bits; f32 rows are multiplied as two float16 terms (22
- * bits), so that the result is as good as 32-bit products'. */
+ * sums are held in 32 bits; f32 rows of q, and the weights whatever the rows'
+ * type, are multiplied as two float16 terms (22 bits), so that the result is as
+ * good as 32-bit products'. */
 typedef struct spt_attention_config {
   int64_t heads;      /* query heads, a multiple of kv_heads */
   int64_t window;     /* keys a row sees at most; 0: all */

@@ -26,9 +26,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The work, B = NB blocks of 32 dims, TERMS f16 terms of q and of the softmax
-// weights (2 for f32 rows: 22 bits each; 1 for f16 and bf16 rows), NT blocks
-// of 8 rows.
+// The work, B = NB blocks of 32 dims, TERMS f16 terms of q (2 for f32 rows: 22
+// bits; 1 holds f16 and bf16 rows), two terms of the softmax weights, NT blocks of
+// 8 rows.
 //
 // Within its share of the 16-key tiles (AttnWalk) a CTA's warps take steps of
 // up to KS tiles in turn, each warp with its own ring of bulk copies and its own
@@ -46,9 +46,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // Bound by instructions: 64 f32 sequences of 8,192 tokens, 8 heads of 64 dims
 // and 8 queries each, read 187 MB in 87 us (2.1 TB/s, 0.55 instructions a clock,
 // the ALU 46% busy with codes becoming f16); one bf16 sequence of 131,000 tokens
-// and 128 dims 151 MB in 65 us (2.3 TB/s).  Three CTAs an SM of steps of two
+// and 128 dims 151 MB in 70 us (2.1 TB/s).  Three CTAs an SM of steps of two
 // tiles took 110 us instead of 87, steps of two tiles on two CTAs 92; at 128 dims
-// one CTA an SM takes 65 us, two 77.
+// two CTAs an SM took 18% longer than one.  16-bit rows: one f16 term of the weights
+// instead of two took 82 us instead of 88 at 64 dims, 65 instead of 70 at 128.
 template <int NB, typename IO, int NT>
 struct Attn {
   static constexpr int kTerms = sizeof(IO) == 4 ? 2 : 1;
@@ -59,8 +60,9 @@ struct Attn {
   static constexpr int kRedBytes = kAttnWarps * kRows * (kDim + 2) * 4;
   static constexpr int kSmem = kAttnWarps * kRing > kRedBytes ? kAttnWarps * kRing : kRedBytes;
   static constexpr int kSub = 2;                  // tiles of a step whose weights are taken at once
-  // CTAs on an SM: 16 warps of 128 registers, where that holds the fragments
-  static constexpr int kMinCtas = NB <= 2 && kTerms * NT < 4 ? 2 : 1;
+  // CTAs on an SM: 16 warps of 128 registers, where that holds the fragments (bf16
+  // rows at 64 dims, two row blocks: 143 us on two CTAs with spills, 135 on one)
+  static constexpr int kMinCtas = (NT == 1 ? NB <= 2 : NB == 1 && kTerms == 1) ? 2 : 1;
   static constexpr int kQ = kTerms == 2 ? NT : (NT + 1) / 2;  // A operands of 16 rows
 };
 
@@ -342,20 +344,20 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
           }
         l[nt] += sum.x + sum.y;
       }
-      // O^T += V^T P^T.  With two terms the step's products are summed from
-      // zero and added in f32: the tensor cores' own additions lose bits of a
-      // long sum.
-      [[maybe_unused]] float oc[NT][NB][2][4];
-      if constexpr (TERMS == 2) {
+      // O^T += V^T P^T.  A weight times its value's scale is two f16 terms whatever
+      // the rows' type: one would be 2^-11 of it off, as much as the rounding of an
+      // f16 row, and more where the values nearly cancel.  The step's products are
+      // summed from zero and added in f32: the tensor cores' own additions lose bits
+      // of a long sum.
+      float oc[NT][NB][2][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < NB; ++k)
+        for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) oc[nt][k][m][x] = 0.0f;
-      }
+            for (int x = 0; x < 4; ++x) oc[nt][k][m][x] = 0.0f;
 #pragma unroll
       for (int i = 0; i < KU; ++i) {
         if (!FULL && (i >= n_tiles || !(ok >> i & 1))) continue;
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
           const uint32_t a0[4] = {e0[0], e0[1], e1[0], e1[1]}, a1[4] = {e0[2], e0[3], e1[2], e1[3]};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            [[maybe_unused]] uint32_t hi[2], lo[2];
+            uint32_t hi[2], lo[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float2 p = __fmul2_rn(s[i][nt][h], __half22float2(half2_of(h ? vd.y : vd.x)));
@@ -379,39 +381,29 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
                 if (hidden(nt, i, h, 1)) p.y = 0.0f;
               }
               const __half2 r = __floats2half2_rn(p.x, p.y);
+              const float2 rest = __ffma2_rn(__half22float2(r), make_float2(-1.0f, -1.0f), p);
               hi[h] = bits(r);
-              if constexpr (TERMS == 2) {
-                const float2 rest = __ffma2_rn(__half22float2(r), make_float2(-1.0f, -1.0f), p);
-                lo[h] = pack_half2(rest.x, rest.y);
-              }
+              lo[h] = pack_half2(rest.x, rest.y);
             }
-            if constexpr (TERMS == 2) {
-              mma16816(oc[nt][k][0], a0, lo[0], lo[1]);
-              mma16816(oc[nt][k][1], a1, lo[0], lo[1]);
-              mma16816(oc[nt][k][0], a0, hi[0], hi[1]);
-              mma16816(oc[nt][k][1], a1, hi[0], hi[1]);
-            } else {
-              // one term: 2^-11 of each weight at most, no more than the rounding of f16 and bf16 rows
-              mma16816(o[nt][k][0], a0, hi[0], hi[1]);
-              mma16816(o[nt][k][1], a1, hi[0], hi[1]);
-            }
+            mma16816(oc[nt][k][0], a0, lo[0], lo[1]);
+            mma16816(oc[nt][k][1], a1, lo[0], lo[1]);
+            mma16816(oc[nt][k][0], a0, hi[0], hi[1]);
+            mma16816(oc[nt][k][1], a1, hi[0], hi[1]);
           }
         }
       }
-      if constexpr (TERMS == 2) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < NB; ++k)
+        for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
-              for (int x = 0; x < 4; x += 2) {
-                const float2 v = __fadd2_rn(make_float2(o[nt][k][m][x], o[nt][k][m][x + 1]),
-                                            make_float2(oc[nt][k][m][x], oc[nt][k][m][x + 1]));
-                o[nt][k][m][x] = v.x, o[nt][k][m][x + 1] = v.y;
-              }
-      }
+            for (int x = 0; x < 4; x += 2) {
+              const float2 v = __fadd2_rn(make_float2(o[nt][k][m][x], o[nt][k][m][x + 1]),
+                                          make_float2(oc[nt][k][m][x], oc[nt][k][m][x + 1]));
+              o[nt][k][m][x] = v.x, o[nt][k][m][x + 1] = v.y;
+            }
     };
 #pragma unroll 1
     for (; read < tb; read += W * per_step) {

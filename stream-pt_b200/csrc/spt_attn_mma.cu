@@ -15,9 +15,11 @@
 //   softmax    one row a thread: the weights 2^(s - ref) of S's row back into
 //              TMEM as f16 terms, O's row added up in registers
 //
-// f32 rows take two f16 terms of q and of the weights: S = Qlo Khi + Qhi Klo +
-// Qhi Khi and O likewise, every product but lo * lo (2^-22 of it); f16 and
-// bf16 rows one term, Q Klo + Q Khi.  O starts from zero for each tile and is
+// f32 rows take two f16 terms of q: S = Qlo Khi + Qhi Klo + Qhi Khi, every product
+// but lo * lo (2^-22 of it); f16 and bf16 rows are one term, S = Q Klo + Q Khi.  The
+// weights are two terms whatever the rows' type, O = Plo Vhi + Phi Vlo + Phi Vhi:
+// one would be 2^-11 of a weight off, as much as the rounding of an f16 row, and
+// more where the values nearly cancel.  O starts from zero for each tile and is
 // added in f32: the tensor cores' own long sums lose bits.  S is double
 // buffered, so that the next tile's products run under a tile's softmax.
 //
@@ -41,7 +43,7 @@ constexpr int kMmaHead = 3;                   // an item's beginning and end, in
 template <int NB, typename IO>
 struct MmaTile {
   static constexpr int kDim = NB * 32;
-  static constexpr int kTerms = sizeof(IO) == 4 ? 2 : 1;        // f16 terms of q and of the weights
+  static constexpr int kTerms = sizeof(IO) == 4 ? 2 : 1;        // f16 terms of q
   static constexpr int kM = NB <= 2 ? 2 : 1;                    // 128-row MMAs of a CTA: a row's O fills the registers above
   static constexpr int kRows = kM * kMmaRows;
   static constexpr int kSoftmaxWarps = 4 * kM;
@@ -437,10 +439,10 @@ __device__ __forceinline__ bool issue(const AttnArgs &a, MmaCta<NB, IO> &s, uint
         const uint32_t o = tmem + m * T::kColsM + T::kColO, p = tmem + m * T::kColsM + (turn & 1) * kMmaKeys;
         // the weights of 16 keys: 8 columns of each term, side by side
 #pragma unroll 1
-        for (int x = 3 - T::kTerms - 1; x < 3; ++x) {  // Plo Vhi (two terms), Phi Vlo, Phi Vhi
+        for (int x = 0; x < 3; ++x) {  // Plo Vhi, Phi Vlo, Phi Vhi
           const uint32_t pt = p + (x == 0 ? 8 : 0), vt = v + (x == 1 ? T::kVTerm / 16 : 0);
 #pragma unroll
-          for (int k = 0; k < kMmaKeys / 16; ++k) mma_ts(leader, o, pt + k * 16, vt + k * 2, o_desc, x + k > 2 - T::kTerms);
+          for (int k = 0; k < kMmaKeys / 16; ++k) mma_ts(leader, o, pt + k * 16, vt + k * 2, o_desc, x + k > 0);
         }
         tc_commit(leader, &s.o_full[m]);
       }
@@ -651,18 +653,14 @@ __device__ __forceinline__ bool softmax(const AttnArgs &a, MmaCta<NB, IO> &s, ui
             float2 p = __ffma2_rn(make_float2(v[16 * q + 2 * x], v[16 * q + 2 * x + 1]), scale2, ref2);
             p.x = exp2_fast(p.x), p.y = exp2_fast(p.y);
             sum = __fadd2_rn(sum, p);
-            if constexpr (T::kTerms == 2) {
-              const float2 f = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xffffe000u),
-                                           __uint_as_float(__float_as_uint(p.y) & 0xffffe000u));
-              const float2 low = __ffma2_rn(f, minus, p);
-              ph[x] = pack_half2(f.x, f.y);
-              pl[x] = pack_half2(low.x, low.y);
-            } else {
-              ph[x] = pack_half2(p.x, p.y);
-            }
+            const float2 f = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xffffe000u),
+                                         __uint_as_float(__float_as_uint(p.y) & 0xffffe000u));
+            const float2 low = __ffma2_rn(f, minus, p);
+            ph[x] = pack_half2(f.x, f.y);
+            pl[x] = pack_half2(low.x, low.y);
           }
           tmem_store8(sc + 16 * q, ph);
-          if constexpr (T::kTerms == 2) tmem_store8(sc + 16 * q + 8, pl);
+          tmem_store8(sc + 16 * q + 8, pl);
         }
         l += sum.x + sum.y;
         tmem_store_wait();
