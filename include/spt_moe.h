@@ -489,7 +489,9 @@ spt_status spt_kv_read_device(spt_context *ctx, spt_kv_cache *cache, int64_t lay
  * of q with a NaN or an infinity gives NaNs and touches no other row.  The
  * sums are held in 32 bits; f32 rows of q, and the weights whatever the rows'
  * type, are multiplied as two float16 terms (22 bits), so that the result is as
- * good as 32-bit products'. */
+ * good as 32-bit products', except that a weighted value is held to 2^-31 of the
+ * largest value that its row sees.  Tokens that a row does not see, stale ones in
+ * the rest of a page included, have no part in its result, whatever they are. */
 typedef struct spt_attention_config {
   int64_t heads;      /* query heads, a multiple of kv_heads */
   int64_t window;     /* keys a row sees at most; 0: all */

@@ -178,10 +178,13 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[nt][k][m][j] = 0.0f;
-    // values' scales seen so far are at most 2^vexp; a weight stands for
-    // 2^(s - ref) with ref = max + vexp - 7, so weight * scale stays within
-    // f16 until a later key exceeds the maximum by 2^8
-    int vexp = -24;
+    // the scales of the values that a row has seen are at most 2^vexp; a weight
+    // stands for 2^(s - ref) with ref = max + vexp - 7, so weight * scale stays
+    // within f16 until a later key exceeds the maximum by 2^8.  Keys that the row
+    // does not see count for nothing: a page's tail may hold anything.
+    int vexp[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) vexp[nt] = -24;
 
     // ---- steps ------------------------------------------------------------------
     // step j of this warp: tiles ta + (warp + j W) per_step on.  Lane i of it looks
@@ -230,7 +233,8 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
       constexpr bool FULL = decltype(full_step)::value;
       // S = Q K^T of the step, and the largest value scale of it
       float2 s[KU][NT][2];  // of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
-      uint32_t vmax = 0;
+      // the largest value scales: of these four keys each, or of all where all are seen
+      uint32_t vmax[FULL ? 1 : KU][FULL ? 1 : 2] = {};
 #pragma unroll
       for (int i = 0; i < KU; ++i) {
 #pragma unroll
@@ -241,7 +245,13 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
         for (int k = 0; k < NB; ++k) {
           const uint2 kd = *reinterpret_cast<const uint2 *>(tile + kv_key_scales(NB) + t * NB * 8 + k * 8);
           const uint2 vd = *reinterpret_cast<const uint2 *>(tile + kv_value_scales(NB) + t * NB * 8 + k * 8);
-          vmax = bits(__hmax2(half2_of(vmax), __hmax2(half2_of(vd.x & 0x7fff7fffu), half2_of(vd.y & 0x7fff7fffu))));
+          const __half2 v0 = half2_of(vd.x & 0x7fff7fffu), v1 = half2_of(vd.y & 0x7fff7fffu);
+          if constexpr (FULL) {
+            vmax[0][0] = bits(__hmax2(half2_of(vmax[0][0]), __hmax2(v0, v1)));
+          } else {
+            vmax[i][0] = bits(__hmax2(half2_of(vmax[i][0]), v0));
+            vmax[i][1] = bits(__hmax2(half2_of(vmax[i][1]), v1));
+          }
           const uint2 word = *reinterpret_cast<const uint2 *>(tile + kv_word(NB, k, lane, 0));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -270,37 +280,41 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
         return key < key_lo[nt] || key >= key_hi[nt] || i >= n_tiles || !(ok >> i & 1);
       };
       // s becomes log2 of the weight
+      float vtop[NT];  // the largest value scale of this lane's keys that its row sees
+      const float2 vm = __half22float2(half2_of(vmax[0][0]));
       bool high = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float2 scale = make_float2(cs[nt], cs[nt]), off = make_float2(-ref[nt], -ref[nt]);
         float top = -INFINITY;
+        vtop[nt] = FULL ? fmaxf(vm.x, vm.y) : 0.0f;
 #pragma unroll
         for (int i = 0; i < KU; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float2 v = __ffma2_rn(s[i][nt][h], scale, off);
-            if (!FULL) {
+            if constexpr (!FULL) {
+              const float2 d = __half22float2(half2_of(vmax[i][h]));
               if (hidden(nt, i, h, 0)) v.x = -INFINITY;
+              else vtop[nt] = fmaxf(vtop[nt], d.x);
               if (hidden(nt, i, h, 1)) v.y = -INFINITY;
+              else vtop[nt] = fmaxf(vtop[nt], d.y);
             }
             s[i][nt][h] = v;
             top = fmaxf(top, fmaxf(v.x, v.y));
           }
-        high |= top > (fresh[nt] ? -INFINITY : (float)(15 - vexp));
+        high |= top > (fresh[nt] ? -INFINITY : (float)(15 - vexp[nt]));
+        high |= vtop[nt] > __uint_as_float((uint32_t)(vexp[nt] + 127) << 23);
       }
-      const float2 vm = __half22float2(half2_of(vmax));
-      const float vtop = fmaxf(vm.x, vm.y);
-      high |= vtop > __uint_as_float((uint32_t)(vexp + 127) << 23);
       if (__any_sync(0xffffffffu, high)) {  // a new maximum: rare after the first steps
-        float vw = vtop;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) vw = fmaxf(vw, __shfl_xor_sync(0xffffffffu, vw, m));
-        int ve = (int)(__float_as_uint(vw) >> 23) - 126;  // vw < 2^ve
-        if (ve > 17) ve = 17;                             // an infinite scale: not written by append
-        if (ve < vexp) ve = vexp;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          float vw = vtop[nt];
+          vw = fmaxf(vw, __shfl_xor_sync(0xffffffffu, vw, 1));
+          vw = fmaxf(vw, __shfl_xor_sync(0xffffffffu, vw, 2));
+          int ve = (int)(__float_as_uint(vw) >> 23) - 126;  // vw < 2^ve
+          if (ve > 17) ve = 17;                             // an infinite scale: not written by append
+          if (ve < vexp[nt]) ve = vexp[nt];
           float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < KU; ++i)
@@ -308,10 +322,13 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
             for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(s[i][nt][h].x, s[i][nt][h].y));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // (a row whose own maxima stand keeps its reference, whatever the others')
+          const bool up = top > (fresh[nt] ? -INFINITY : (float)(15 - vexp[nt])) ||
+                          vw > __uint_as_float((uint32_t)(vexp[nt] + 127) << 23);
           float most = top + ref[nt];
-          if (!fresh[nt]) most = fmaxf(most, ref[nt] - (float)(vexp - 7));
+          if (!fresh[nt]) most = fmaxf(most, ref[nt] - (float)(vexp[nt] - 7));
           const bool none = most == -INFINITY;
-          const float now = none ? 0.0f : most + (float)(ve - 7);
+          const float now = !up ? ref[nt] : none ? 0.0f : most + (float)(ve - 7);
           const float factor = fresh[nt] ? 1.0f : exp2f(ref[nt] - now);
           const float2 move = make_float2(ref[nt] - now, ref[nt] - now);
 #pragma unroll
@@ -321,6 +338,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
           l[nt] *= factor;
           ref[nt] = now;
           fresh[nt] = none;
+          if (up) vexp[nt] = ve;
           const float f0 = __shfl_sync(0xffffffffu, factor, 8 * t), f1 = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
 #pragma unroll
           for (int k = 0; k < NB; ++k)
@@ -330,7 +348,6 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
               o[nt][k][m][2] *= f0, o[nt][k][m][3] *= f1;
             }
         }
-        vexp = ve;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {

@@ -124,9 +124,10 @@ __device__ __forceinline__ SeqRows seq_rows(const AttnArgs &a, int64_t b) {
 }
 
 // Tiles of KEYS keys, [first, last), that row block rb of a sequence sees: a
-// block is ROWS consecutive (new row, head of the group) pairs.
+// block is ROWS consecutive (new row, head of the group) pairs.  [lo, hi) are the
+// keys that any of its rows sees.
 struct KeyTiles {
-  int first, last;
+  int first, last, lo, hi;
 };
 template <int ROWS, int KEYS>
 __device__ __forceinline__ KeyTiles key_tiles(const AttnArgs &a, const SeqRows &s, int rb) {
@@ -139,8 +140,8 @@ __device__ __forceinline__ KeyTiles key_tiles(const AttnArgs &a, const SeqRows &
   if (hi > cap) hi = cap;
   int64_t lo = a.window > 0 ? (int64_t)s.len - s.n + i0 - a.window + 1 : 0;
   if (lo < 0) lo = 0;
-  KeyTiles t = {0, 0};
-  if (hi > lo) t.first = (int)(lo / KEYS), t.last = (int)((hi + KEYS - 1) / KEYS);
+  KeyTiles t = {0, 0, 0, 0};
+  if (hi > lo) t.first = (int)(lo / KEYS), t.last = (int)((hi + KEYS - 1) / KEYS), t.lo = (int)lo, t.hi = (int)hi;
   return t;
 }
 template <int ROWS>

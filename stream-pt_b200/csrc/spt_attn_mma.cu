@@ -10,7 +10,9 @@
 //              looks at their scales
 //   dequant    six warps, write keys and values as f16 pairs hi + lo: a code
 //              times its scale has 15 bits, so hi + lo is exact (a power of two
-//              for the tile, its largest scale's, keeps both in f16's range)
+//              for the tile brings the largest scale that a row of the CTA sees to
+//              2^11; scales down to 2^-25 of it keep all their bits, smaller ones
+//              are at most 2^-36 of it off).  What no row sees is written as zeros.
 //   issuer     S = Q K^T and O = P V into TMEM, from Q and P in TMEM, 128 rows each
 //   softmax    one row a thread: the weights 2^(s - ref) of S's row back into
 //              TMEM as f16 terms, O's row added up in registers
@@ -164,8 +166,15 @@ struct TileInfoAttn {
 struct RawInfo {
   float k_up, v_up;
   uint32_t ok;
-  int end;  // no tile: there are no more
+  int end;     // no tile: there are no more
+  int lo, hi;  // the loader's: keys [lo, hi) of the tile are seen by rows of the item
 };
+
+// The scales of tokens `token`, + 1, + 8 and + 9 of a tile, zero outside [lo, hi).
+__device__ __forceinline__ uint2 seen_scales(uint2 d, int token, int lo, int hi) {
+  auto pair = [&](int t) { return (t >= lo && t < hi ? 0xffffu : 0u) | (t + 1 >= lo && t + 1 < hi ? 0xffff0000u : 0u); };
+  return make_uint2(d.x & pair(token), d.y & pair(token + 8));
+}
 
 // A tile's information is overwritten by that of the tile kInfos on, which is
 // loaded when the raw slot kRaw tiles before it is free, that is behind the PV
@@ -214,7 +223,7 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, MmaCta<NB, IO> &s,
   int at = w.first_tile(), last = w.last_tile();
   bool more = true, page_known = false;
   int32_t page = 0;
-  uint32_t oks = 0;            // 4 bits a tile under way: the oldest lowest
+  uint32_t oks = 0;            // 4 bits a tile under way, and one more where keys of it are seen by no row: the oldest lowest
   int ahead = 0, put = 0, get = 0, left_out = -1;
   uint32_t put_phase = 0, get_phase = 0, jt = 0;
   // starts the next tile's copies; false where a wait gave up
@@ -238,7 +247,10 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, MmaCta<NB, IO> &s,
       bulk_load(raw + put * T::kRawTile + lane * T::kRecord,
                 a.c.base + kv_tile_offset(a.c, page, w.head, (int)place * kKvTile), T::kRecord, &s.raw_full[put]);
     }
-    oks |= ok << (4 * ahead);
+    const int lo = w.tiles.lo - at * kMmaKeys, hi = w.tiles.hi - at * kMmaKeys;
+    const bool edge = lo > 0 || hi < kMmaKeys;
+    if (edge && lane == 0) s.raw[put].lo = lo, s.raw[put].hi = hi;
+    oks |= (ok | (edge ? 16u : 0u)) << (5 * ahead);
     if (++put == T::kRaw) put = 0, put_phase ^= 1u;
     ++ahead;
     page = page_of(++at);  // of the item's next tile, if it has one
@@ -252,7 +264,18 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, MmaCta<NB, IO> &s,
   while (fine && ahead > 0) {
     if (!warp_wait(&s.raw_full[get], get_phase, a, 43)) break;
     const uint32_t ok = oks & 15u;
-    const uint8_t *from = raw + get * T::kRawTile;
+    uint8_t *from = raw + get * T::kRawTile;
+    if (oks & 16u) {  // what no row sees counts as zeros, here and for the dequant warps
+      const int lo = s.raw[get].lo, hi = s.raw[get].hi;
+#pragma unroll 1
+      for (int c = lane; c < 16 * NB; c += 32) {
+        const int sub = c / (4 * NB), token = sub * kKvTile + c % (4 * NB) / NB * 2;
+        uint2 *d = reinterpret_cast<uint2 *>(from + sub * T::kRecord + kv_key_scales(NB) + c % (4 * NB) * 8);
+        d[0] = seen_scales(d[0], token, lo, hi);
+        d[4 * NB] = seen_scales(d[4 * NB], token, lo, hi);  // (the values' come behind the keys')
+      }
+      fence_async_smem();  // the slot's next copy comes behind these writes
+    }
     // largest scales of keys (low half) and values (high), NaNs aside; values' NaNs
     __half2 top = half2_of(0);
     uint32_t nan = 0;
@@ -283,7 +306,7 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, MmaCta<NB, IO> &s,
       info.v_unit = exp2_int(-ve);
       info.ok = ok;
       info.any_nan = any;
-      s.raw[get] = {exp2_int(ke), exp2_int(ve), ok, 0};
+      s.raw[get] = {exp2_int(ke), exp2_int(ve), ok, 0, 0, 0};
     }
     if (any) {
       if (lane < kKvMaxBlocks) info.nan[lane] = 0;
@@ -300,7 +323,7 @@ __device__ __forceinline__ void load_tiles(const AttnArgs &a, MmaCta<NB, IO> &s,
       mbar_arrive(&s.info_full[jt % kInfos]);
     }
     ++jt;
-    oks >>= 4;
+    oks >>= 5;
     --ahead;
     if (++get == T::kRaw) get = 0, get_phase ^= 1u;
     fine = start();

@@ -72,3 +72,63 @@ def test_values_that_nearly_cancel(ctx, type, dim, length, counts):
     off, tol = (out.double() - want[0]).abs(), tolerance(want, length, type)
     assert bool((off <= tol).all()), float((off / tol).max())
     cache.close()
+
+
+@pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("counts", [None, [2, 2], [90, 40]], ids=str)
+@pytest.mark.parametrize("junk", [1e3, 1e6, -6e5])
+def test_large_values_in_masked_places(ctx, type, counts, junk):
+    """Finite numbers of any size behind the length and before the window, beside small values in
+    sight, change no bit: neither of single rows nor of chunks."""
+    import torch
+    lengths, whole = [300, 200], [320, 256]
+    n = [1, 1] if counts is None else counts
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    table, _, pages = random_table(np.random.default_rng(3), whole, 32)
+    cache = ctx.kv_cache(kv_heads=2, head_dim=64, page_tokens=32, pages=pages)
+    k = torch.randn(500, 2, 64, generator=gen, device="cuda")
+    v = 1e-3 * torch.randn(500, 2, 64, generator=gen, device="cuda")
+    append(ctx, cache, table, lengths, lengths, k, v)
+    held = [read(ctx, cache, table[b:b + 1], lengths[b]) for b in range(2)]
+    q = torch.randn(sum(n), 16, 64, generator=gen, device="cuda").to(torch_type(type))
+    window = 37
+    want, seen = attend(ctx, cache, table, lengths, counts, q), attend(ctx, cache, table, lengths, counts, q, window)
+    at = 0
+    for b, c in enumerate(n):
+        for out, w in ((want, 0), (seen, window)):
+            exact = attention(q[at:at + c].double(), *held[b], lengths[b] - c, 0.125, w)
+            assert bool(((out[at:at + c].double() - exact[0]).abs() <= tolerance(exact, lengths[b], type)).all())
+        at += c
+    # behind the lengths
+    tail = [w - m for w, m in zip(whole, lengths)]
+    x = torch.full((sum(tail), 2, 64), junk, device="cuda")
+    append(ctx, cache, table, whole, tail, x, x)
+    assert bool((attend(ctx, cache, table, lengths, counts, q) == want).all())
+    assert bool((attend(ctx, cache, table, lengths, counts, q, window) == seen).all())
+    # and up to the first key that a row with the window sees
+    head = [m - c + 1 - window for m, c in zip(lengths, n)]
+    x = torch.full((sum(head), 2, 64), junk, device="cuda")
+    append(ctx, cache, table, head, head, x, x)
+    assert bool((attend(ctx, cache, table, lengths, counts, q, window) == seen).all())
+    cache.close()
+
+
+@pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("count", [2, 60])
+def test_a_later_token_stays_out_of_earlier_rows(ctx, type, count):
+    """The last token's key and value change, up to 2^20 times their neighbours': the rows before it keep every bit."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    length = 150
+    table, _, pages = random_table(np.random.default_rng(4), [length], 16)
+    cache = ctx.kv_cache(kv_heads=2, head_dim=64, page_tokens=16, pages=pages)
+    k = torch.randn(length, 2, 64, generator=gen, device="cuda")
+    v = torch.randn(length, 2, 64, generator=gen, device="cuda")
+    append(ctx, cache, table, [length], [length], k, 1e-2 * v)
+    q = torch.randn(count, 16, 64, generator=gen, device="cuda").to(torch_type(type))
+    want = attend(ctx, cache, table, [length], [count], q)
+    for size in (1.0, 100.0, 1e4):
+        append(ctx, cache, table, [length], [1], -k[:1].contiguous(), size * v[:1])
+        out = attend(ctx, cache, table, [length], [count], q)
+        assert bool((out[:-1] == want[:-1]).all()) and not bool((out[-1] == want[-1]).all())
+    cache.close()
