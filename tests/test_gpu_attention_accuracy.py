@@ -132,3 +132,20 @@ def test_a_later_token_stays_out_of_earlier_rows(ctx, type, count):
         out = attend(ctx, cache, table, [length], [count], q)
         assert bool((out[:-1] == want[:-1]).all()) and not bool((out[-1] == want[-1]).all())
     cache.close()
+
+
+@pytest.mark.parametrize("type", list(TYPES))
+def test_single_tokens_with_and_without_offsets(ctx, type):
+    """The same batch either way, to the last bit."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    lengths = [4000, 3, 900, 1, 77]
+    table, _, pages = random_table(np.random.default_rng(6), lengths, 16)
+    cache = ctx.kv_cache(kv_heads=2, head_dim=64, page_tokens=16, pages=pages)
+    n = sum(lengths)
+    append(ctx, cache, table, lengths, lengths, torch.randn(n, 2, 64, generator=gen, device="cuda"),
+           torch.randn(n, 2, 64, generator=gen, device="cuda"))
+    q = torch.randn(5, 16, 64, generator=gen, device="cuda").to(torch_type(type))
+    a, b = attend(ctx, cache, table, lengths, None, q), attend(ctx, cache, table, lengths, [1] * 5, q)
+    assert bool((a == b).all())
+    cache.close()
