@@ -236,8 +236,9 @@ spt_status spt_context_set_path(spt_context *ctx, int path);
  *                         for it runs out (the failure path without a fault);
  *                         1000: the shared-memory router's CTA 0 leaves out
  *                         one row's copy, so its wait runs out; in
- *                         spt_attention's many-row kernel CTA 0 leaves out
- *                         this tile's copies
+ *                         spt_attention CTA 0 leaves out the copies of this
+ *                         tile (many rows) or of its first warp's this step
+ *                         (few rows)
  *   SPT_OPT_HOST_GRAPHS   1 (default): spt_forward_moe_batch / spt_forward_moe
  *                         capture the block's kernels into a CUDA graph on the
  *                         second call with the same arena, layer, batch and

@@ -96,6 +96,11 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
   const uint32_t tiles_per_page = (uint32_t)a.c.page_tokens / kKvTile;
   int stage = 0;  // of this warp's ring: the step to be read next
   uint32_t phase = 0;
+  // A warp whose wait runs out takes no more steps: it waits for its copies in
+  // flight, whose bytes would else land in the sums that follow or in another CTA's
+  // shared memory, and comes to the meetings and the arrivals as the others do.
+  bool gave_up = false;
+  uint32_t steps = 0;  // that this warp has asked for
   do {
     const SeqRows &seq = w.seq;
     const int rb = w.rb, ta = w.first_tile(), tb = w.last_tile();  // tiles [ta, tb) of the item are this CTA's
@@ -201,8 +206,13 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
       place = tile - p * tiles_per_page;
       page = lane < per_step && (int)tile < tb ? __ldcg(pages + p) : -1;
     };
+    int left_out = -1;
     auto fetch = [&](int to) {  // the step that was asked for, into ring slot `to`
       const bool good = page >= 0 && page < a.c.pages;
+      if (blockIdx.x == 0 && warp == 0 && steps++ == (uint32_t)a.fault_tile) {
+        left_out = to;
+        return 0u;
+      }
       const uint32_t ok = __ballot_sync(0xffffffffu, good);
       const uint32_t starts = __ballot_sync(0xffffffffu, good && (place == 0 || lane == 0 || !(ok >> (lane - 1) & 1)));
       if (lane == 0) mbar_expect_tx(&bars[warp][to], __popc(ok) * TILE);
@@ -216,7 +226,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
     };
     uint32_t ok_now = 0, ok_next = 0;  // good pages of the steps under way
     int slot = stage;
-    if (asked < tb) {
+    if (asked < tb && !gave_up) {
       ask(asked);
       ok_now = fetch(slot);
       asked += W * per_step;
@@ -423,8 +433,14 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
             }
     };
 #pragma unroll 1
-    for (; read < tb; read += W * per_step) {
-      brief_wait(&bars[warp][stage], phase, a, 46);  // (this warp's own copies; a wait that gives up is reported)
+    for (; read < tb && !gave_up; read += W * per_step) {
+      if (!__all_sync(0xffffffffu, own_wait(&bars[warp][stage], phase, a, 46))) {
+        gave_up = true;  // the step of this slot and the next are in flight
+        if (stage != left_out) mbar_wait_own(&bars[warp][stage], phase);
+        if (++stage == kAttnStages) stage = 0, phase ^= 1u;
+        if (read + W * per_step < tb && stage != left_out) mbar_wait_own(&bars[warp][stage], phase);
+        break;
+      }
       __syncwarp();  // the slot read last is free: the step after the next goes there
       uint32_t ok_then = 0;
       if (asked < tb) ok_then = fetch(slot);

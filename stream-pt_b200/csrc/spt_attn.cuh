@@ -99,6 +99,20 @@ __device__ __forceinline__ bool brief_wait(uint64_t *bar, uint32_t parity, const
   }
 }
 
+// The same for copies that the calling warp started itself: nothing that happens
+// elsewhere, in this launch or an earlier one, ends it before its time.
+__device__ __forceinline__ bool own_wait(uint64_t *bar, uint32_t parity, const AttnArgs &a, int code) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 63u) == 0u && clock64() - t0 > (1ll << a.wait_shift)) {
+      atomicCAS(a.err, 0, code);
+      return false;
+    }
+  }
+}
+
 // a / b for non-negative a, which seldom need 64 bits.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);

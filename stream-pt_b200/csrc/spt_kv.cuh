@@ -120,7 +120,7 @@ struct AttnArgs {
   int32_t *arrive = nullptr;     // attn_counters() zeros between launches
   int32_t *err = nullptr;        // set when a bounded wait gives up
   int wait_shift = 31;
-  int fault_tile = -1;           // a test's: CTA 0 leaves out this tile's copies
+  int fault_tile = -1;           // a test's: CTA 0 leaves out this tile's (its first warp's step's) copies
   int sm_count = 148;
 };
 cudaError_t launch_attention(const AttnArgs &a, cudaStream_t stream);
