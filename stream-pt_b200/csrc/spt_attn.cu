@@ -571,12 +571,14 @@ cudaError_t launch_dims(const AttnArgs &a, cudaStream_t stream) {
 size_t attn_workspace_bytes(int sm_count, int nb) {
   return (size_t)sm_count * kAttnCtasPerSm * 2 * 16 * (nb * 32 + 2) * sizeof(float);
 }
-size_t attn_counter_bytes(int sm_count) { return (size_t)sm_count * kAttnCtasPerSm * sizeof(int32_t); }
+// a counter a CTA, and a flag for each CTA of the many-row kernel
+size_t attn_counter_bytes(int sm_count) { return (size_t)sm_count * (kAttnCtasPerSm + 1) * sizeof(int32_t); }
 
 cudaError_t launch_attention(const AttnArgs &args, cudaStream_t stream) {
   AttnArgs a = args;
   if (a.r.tokens <= 0 || a.r.sequences <= 0) return cudaSuccess;
   if (a.r.tokens > INT32_MAX / a.group) return cudaErrorInvalidValue;
+  a.gave_up = a.arrive + a.sm_count * kAttnCtasPerSm;
   const int size = a.type == kKvF32 ? 4 : 2;
   a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * size)) & 15) == 0;
   a.out_vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * size)) & 15) == 0;

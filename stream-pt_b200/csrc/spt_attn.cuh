@@ -82,25 +82,27 @@ __device__ __forceinline__ void store_row4(IO *p, bool vec, const float (&x)[4])
   }
 }
 
-// mbar_wait for waits that are short as a rule: the error flag lies in global
-// memory, so it and the clock are looked at every 64th try only.
+// A bounded wait for another role of this CTA, short as a rule: the clock and the
+// CTA's word for a role that has given up are looked at every 64th try only (an
+// error that an earlier call left in a.err ends no wait of this one; the CTA
+// records its own there in the end).  One atomic here keeps the sites short: a flag
+// in shared memory beside a.err took f16 chunks of 12 sequences from 227 to 245 us.
 __device__ __forceinline__ bool brief_wait(uint64_t *bar, uint32_t parity, const AttnArgs &a, int code) {
   if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
   for (uint32_t i = 1;; ++i) {
     if (mbar_try(bar, parity)) return true;
     if ((i & 63u) == 0u) {
-      if (*(volatile int32_t *)a.err != 0) return false;  // another role already gave up
+      if (*(volatile int32_t *)(a.gave_up + blockIdx.x)) return false;
       if (clock64() - t0 > (1ll << a.wait_shift)) {
-        atomicCAS(a.err, 0, code);
+        atomicCAS(a.gave_up + blockIdx.x, 0, code);
         return false;
       }
     }
   }
 }
 
-// The same for copies that the calling warp started itself: nothing that happens
-// elsewhere, in this launch or an earlier one, ends it before its time.
+// The same for copies that the calling warp started itself.
 __device__ __forceinline__ bool own_wait(uint64_t *bar, uint32_t parity, const AttnArgs &a, int code) {
   if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();

@@ -796,6 +796,7 @@ __global__ void __launch_bounds__(MmaTile<NB, IO>::kThreads, 1) k_attn_mma(const
   MmaWalk<NB, IO> w;
   if (!w.template begin<T::kThreads>(a, kMmaMinTiles, blockIdx.x, gridDim.x)) return;
   if (threadIdx.x == 0) {
+    a.gave_up[blockIdx.x] = 0;
     for (int i = 0; i < T::kRaw; ++i) {
       mbar_init(&s.raw_full[i], 1);
       mbar_init(&s.raw_ready[i], 1);
@@ -857,6 +858,10 @@ __global__ void __launch_bounds__(MmaTile<NB, IO>::kThreads, 1) k_attn_mma(const
   tc_before();
   __syncthreads();
   tc_after();
+  if (threadIdx.x == 0) {
+    const int code = *(volatile int32_t *)(a.gave_up + blockIdx.x);
+    if (code != 0) atomicCAS(a.err, 0, code);
+  }
   if (warp == T::kSoftmaxWarps)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(T::kCols) : "memory");
 }

@@ -117,7 +117,8 @@ struct AttnArgs {
   int type = kKvF32;
   bool q_vec = false, out_vec = false;  // rows start on 16 bytes
   float *partial = nullptr;      // attn_workspace_bytes()
-  int32_t *arrive = nullptr;     // attn_counters() zeros between launches
+  int32_t *arrive = nullptr;     // attn_counter_bytes(): counters, zero between launches
+  int32_t *gave_up = nullptr;    // the many-row kernel's, behind them: a word a CTA, set when one of its waits gives up
   int32_t *err = nullptr;        // set when a bounded wait gives up
   int wait_shift = 31;
   int fault_tile = -1;           // a test's: CTA 0 leaves out this tile's (its first warp's step's) copies

@@ -67,3 +67,23 @@ def test_single_tokens_behind_a_call_that_gave_up(ctx):
         reported(ctx)
     assert bool((got == want).all())
     cache.close()
+
+
+def test_many_rows_behind_a_call_that_gave_up(ctx):
+    """The same for chunks of rows, of which every CTA waits for copies and for its other warps."""
+    import torch
+    lengths, counts = [3000, 700], [300, 64]
+    cache, table, held = filled(ctx, 23, lengths, 2, 64, 16)
+    q, out = torch.randn(364, 16, 64, device="cuda"), torch.zeros(364, 16, 64, device="cuda")
+    dev = Device(table, lengths, counts)
+    want = check(ctx, cache, table, held, lengths, counts, 16, scale=0.125, q=q)
+    got = torch.zeros_like(want)
+    torch.cuda.synchronize()
+    with short_waits(ctx):
+        ctx.set_option(spt.OPT_FAULT_STAGE, 2)
+        cache.attention_device(dev.batch, q.data_ptr(), out.data_ptr(), 16, scale=0.125)
+        ctx.set_option(spt.OPT_FAULT_STAGE, -1)
+        cache.attention_device(dev.batch, q.data_ptr(), got.data_ptr(), 16, scale=0.125)
+        reported(ctx)
+    assert bool((got == want).all())
+    cache.close()
