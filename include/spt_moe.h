@@ -548,7 +548,9 @@ spt_status spt_beam_select(spt_context *ctx, spt_beam *beam, const float *logits
  * pages are distinct and in no table.  A parent outside [0, beams) leaves an
  * empty sequence.  table_out (entries behind the last page -1), lengths_out
  * and copied (1 where the spare page was taken; may be NULL) do not overlap
- * the inputs.  Device pointers; pages outside the pool are not copied. */
+ * the inputs.  Device pointers; a last page outside the pool is not copied, and
+ * every child has its number.  A spare page outside the pool, where one is
+ * needed, leaves its child an entry that no call reads. */
 spt_status spt_kv_reorder_device(spt_context *ctx, spt_kv_cache *cache, int64_t batch, int64_t beams,
                                  int64_t max_pages, const int32_t *parents, int64_t parents_stride,
                                  const int32_t *table, const int32_t *lengths, const int32_t *spare,

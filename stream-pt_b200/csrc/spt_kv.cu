@@ -424,8 +424,10 @@ __global__ void __launch_bounds__(kKvThreads) k_kv_reorder(uint8_t *pool, int64_
   bool later = false;
   for (int64_t i = 0; i < j; ++i) later |= parents[i] == parent;
   const int64_t old = rest ? a.table[from * a.max_pages + full] : -1;
-  const int64_t own = later ? a.spare[s] : old;
-  const bool copy = rest && later && old >= 0 && old < c.pages && own >= 0 && own < c.pages;
+  // a page outside the pool has nothing to copy: every child keeps its number, and no spare page is taken
+  const bool held = old >= 0 && old < c.pages;
+  const int64_t own = later && held ? a.spare[s] : old;
+  const bool copy = rest && later && held && own >= 0 && own < c.pages;
   if (blockIdx.y == 0) {
     for (int64_t i = threadIdx.x; i < a.max_pages; i += kKvThreads)
       a.table_out[s * a.max_pages + i] =
