@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
       const int r = rb * ROWS + nt * 8 + g, i = (int)((uint32_t)r / (uint32_t)a.group);
       const bool live = i < seq.n;
       const int qh = head * a.group + r - i * a.group;
-      key_hi[nt] = live ? seq.len - seq.n + i + 1 : 0;
+      key_hi[nt] = live ? max(seq.len - seq.n + i + 1, 0) : 0;
       key_lo[nt] = a.window > 0 && key_hi[nt] > a.window ? key_hi[nt] - (int)a.window : 0;
       if (live) {
         all_lo = key_lo[nt] > all_lo ? key_lo[nt] : all_lo;
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn<NB, IO, NT>::kMinCtas) k_at
 #pragma unroll 1
       for (; n_tiles > 0; n_tiles -= KU, key0 += KU * kKvTile, buf += KU * TILE, ok >>= KU) {
         constexpr uint32_t all = (1u << KU) - 1u;
-        if (n_tiles >= KU && (ok & all) == all && key0 >= all_lo && key0 + KU * kKvTile <= all_hi)
+        if (n_tiles >= KU && (ok & all) == all && key0 >= all_lo && all_hi - key0 >= KU * kKvTile)
           step(std::true_type{}, buf, key0, KU, all);
         else
           step(std::false_type{}, buf, key0, n_tiles, ok);

@@ -523,8 +523,8 @@ __device__ __forceinline__ bool softmax(const AttnArgs &a, MmaCta<NB, IO> &s, ui
     const bool live = i < seq.n;
     const int head = w.head * a.group + r - i * a.group;
     const int first = w.first_tile(), last = w.last_tile();
-    // positions are below 2^31
-    const int key_hi = live ? seq.len - seq.n + i + 1 : 0;
+    // positions are below 2^31, a tile's end may not be
+    const int key_hi = live ? max(seq.len - seq.n + i + 1, 0) : 0;
     const int key_lo = a.window > 0 && key_hi > a.window ? key_hi - (int)a.window : 0;
     float ref = 0.0f, l = 0.0f;
     bool fresh = true;
@@ -629,7 +629,7 @@ __device__ __forceinline__ bool softmax(const AttnArgs &a, MmaCta<NB, IO> &s, ui
         // (never 0: a masked score of -inf has to stay one)
         const float scale = fmaxf(c * info.k_unit, 1.2e-38f), next_unit = info.v_unit;
         const uint32_t ok = info.ok, any_nan = info.any_nan;
-        const bool edge = __any_sync(0xffffffffu, key_lo > key0 || key_hi < key0 + kMmaKeys || ok != 15u);
+        const bool edge = __any_sync(0xffffffffu, key_lo > key0 || key_hi - key0 < kMmaKeys || ok != 15u);
         float v[kMmaKeys];
         tmem_load(sc, v);
         if (edge || any_nan) {  // keys of the tile that this row does not see: their scores become -inf
