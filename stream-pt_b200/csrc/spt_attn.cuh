@@ -356,7 +356,7 @@ __device__ __forceinline__ float row_factor(const AttnArgs &a, int head, float r
       up = exp2f(ref - top);
       below = l * up + exp2f(sink - top);
     }
-    if (isnan(sink)) below = sink;
+    if (!(sink < INFINITY)) below = sink;  // (infinite: every weight is 0)
   }
   return below == 0.0f ? 0.0f : up / below;
 }

@@ -42,3 +42,29 @@ def test_lengths_up_to_the_largest(ctx, type, count, short):
     assert bool((back.double() == k2[end - n:end]).all()) and bool((k2[:end - n] == keys[:end - n]).all())
     assert bool((v2[end:] == values[end:]).all())
     cache.close()
+
+
+@pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("counts", [None, [1, 1, 0], [90, 40, 7]], ids=str)
+def test_infinite_sinks(ctx, type, counts):
+    """An infinite sink takes all weight, one of -inf none, a NaN gives NaNs: in that head alone, with keys and
+    without."""
+    import numpy as np
+    import torch
+
+    from kv_plain import random_table
+    inf = float("inf")
+    lengths = [300, 200, 5]
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    table, _, pages = random_table(np.random.default_rng(8), lengths, 16)
+    cache = ctx.kv_cache(kv_heads=2, head_dim=64, page_tokens=16, pages=pages)
+    append(ctx, cache, table, lengths, lengths, torch.randn(505, 2, 64, generator=gen, device="cuda"),
+           torch.randn(505, 2, 64, generator=gen, device="cuda"))
+    n = 3 if counts is None else sum(counts)
+    q = torch.randn(n, 4, 64, generator=gen, device="cuda").to(torch_type(type))
+    plain = attend(ctx, cache, table, lengths, counts, q)
+    out = attend(ctx, cache, table, lengths, counts, q, sinks=torch.tensor([inf, -inf, 3e38, float("nan")], device="cuda"))
+    assert not bool(out[:, 0].any()) and not bool(out[:, 2].any()) and bool(torch.isnan(out[:, 3]).all())
+    off = (out[:, 1].float() - plain[:, 1].float()).abs()  # the same sums, divided by them plus 0
+    assert bool((off <= plain[:, 1].float().abs() * 2.0 ** -22).all()) or type != "f32" and bool((off == 0).all())
+    cache.close()
