@@ -821,22 +821,40 @@ class KvBatch:
     """spt_kv_rows: which rows of a call belong to which sequence, and where
     their tokens lie.  `table` [sequences, max_pages], `lengths` [sequences]
     and `offsets` [sequences + 1] (None or 0: row b is sequence b's one new
-    row) are device addresses for the *_device calls, or int32 arrays for the
-    host calls."""
+    row) are device addresses for the *_device calls, or int32 arrays of at
+    least those sizes for the host calls; a call refuses the other kind."""
 
     def __init__(self, sequences: int, tokens: int, max_pages: int, table, lengths, offsets=None):
-        self._keep = []
+        self._keep, self._addresses = [], 0
 
-        def address(a):
-            if a is None or isinstance(a, int):
-                return a or None
+        def address(a, size, name):
+            if a is None or isinstance(a, (int, np.integer)):
+                self._addresses += bool(a)
+                return int(a) if a else None
             a = np.ascontiguousarray(a, dtype=np.int32)
+            if a.size < size:
+                raise SptError(ERR_DIMENSIONS, f"{name}: {a.size} entries instead of {size}")
             self._keep.append(a)
             return a.ctypes.data
 
-        self.c = _KvRows(sequences, tokens, max_pages, address(table), address(lengths), address(offsets))
+        self.c = _KvRows(sequences, tokens, max_pages, address(table, sequences * max_pages, "page table"),
+                         address(lengths, sequences, "lengths"), address(offsets, sequences + 1, "offsets"))
         self.tokens = tokens
         self.ref = ctypes.byref(self.c)
+
+    @property
+    def host(self):
+        """The rows of a host call."""
+        if self._addresses:
+            raise SptError(ERR_DIMENSIONS, "a host call takes arrays, not device addresses")
+        return self.ref
+
+    @property
+    def device(self):
+        """The rows of a *_device call."""
+        if self._keep:
+            raise SptError(ERR_DIMENSIONS, "a device call takes device addresses, not host arrays")
+        return self.ref
 
 
 class KvCache:
@@ -855,31 +873,31 @@ class KvCache:
 
     def append_device(self, batch: KvBatch, k_ptr: int, v_ptr: int, type: int = GGML_F32, layer: int = 0,
                       k_stride: int = 0, v_stride: int = 0):
-        self.ctx.check(lib().spt_kv_append_device(self.ctx._h, self._h, layer, batch.ref, type, k_ptr, k_stride, v_ptr,
+        self.ctx.check(lib().spt_kv_append_device(self.ctx._h, self._h, layer, batch.device, type, k_ptr, k_stride, v_ptr,
                                                   v_stride))
 
     def read_device(self, batch: KvBatch, k_ptr: int, v_ptr: int, type: int = GGML_F32, layer: int = 0,
                     k_stride: int = 0, v_stride: int = 0):
-        self.ctx.check(lib().spt_kv_read_device(self.ctx._h, self._h, layer, batch.ref, type, k_ptr or None, k_stride,
+        self.ctx.check(lib().spt_kv_read_device(self.ctx._h, self._h, layer, batch.device, type, k_ptr or None, k_stride,
                                                 v_ptr or None, v_stride))
 
     def attention_device(self, batch: KvBatch, q_ptr: int, out_ptr: int, heads: int, type: int = GGML_F32,
                          scale: float = 1.0, window: int = 0, sinks_ptr: int = 0, layer: int = 0, q_stride: int = 0,
                          out_stride: int = 0):
         c = _AttentionConfig(heads, window, scale, sinks_ptr or None)
-        self.ctx.check(lib().spt_attention_device(self.ctx._h, self._h, layer, batch.ref, ctypes.byref(c), type, q_ptr,
+        self.ctx.check(lib().spt_attention_device(self.ctx._h, self._h, layer, batch.device, ctypes.byref(c), type, q_ptr,
                                                   q_stride, out_ptr, out_stride))
 
     def append(self, batch: KvBatch, k: np.ndarray, v: np.ndarray, layer: int = 0, cancel=None):
         k, v = _f32(k), _f32(v)
-        self.ctx.check(lib().spt_kv_append(self.ctx._h, self._h, layer, batch.ref, _p(k), k.size, _p(v), v.size,
+        self.ctx.check(lib().spt_kv_append(self.ctx._h, self._h, layer, batch.host, _p(k), k.size, _p(v), v.size,
                                            _p(cancel)))
 
     def read(self, batch: KvBatch, layer: int = 0, cancel=None):
         """(k, v) [tokens, kv_heads, head_dim] as the cache holds them (0 in rows of no sequence)."""
         shape = (batch.tokens, self.kv_heads, self.head_dim)
         k, v = np.zeros(shape, np.float32), np.zeros(shape, np.float32)
-        self.ctx.check(lib().spt_kv_read(self.ctx._h, self._h, layer, batch.ref, _p(k), k.size, _p(v), v.size,
+        self.ctx.check(lib().spt_kv_read(self.ctx._h, self._h, layer, batch.host, _p(k), k.size, _p(v), v.size,
                                          _p(cancel)))
         return k, v
 
@@ -889,10 +907,14 @@ class KvCache:
         """[tokens, heads, head_dim]; rows of no sequence stay as `out` has them (0 without `out`)."""
         q = _f32(q)
         sinks = None if sinks is None else _f32(sinks)
+        if sinks is not None and sinks.size != heads:
+            raise SptError(ERR_DIMENSIONS, f"{sinks.size} sinks for {heads} heads")
         if out is None:
             out = np.zeros((batch.tokens, heads, self.head_dim), np.float32)
+        if not (isinstance(out, np.ndarray) and out.dtype == np.float32 and out.flags.c_contiguous and out.flags.writeable):
+            raise SptError(ERR_DIMENSIONS, "the output is no contiguous float32 array")
         c = _AttentionConfig(heads, window, scale, None if sinks is None else sinks.ctypes.data)
-        self.ctx.check(lib().spt_attention(self.ctx._h, self._h, layer, batch.ref, ctypes.byref(c), _p(q), q.size,
+        self.ctx.check(lib().spt_attention(self.ctx._h, self._h, layer, batch.host, ctypes.byref(c), _p(q), q.size,
                                            _p(out), out.size, _p(cancel)))
         return out
 
@@ -910,6 +932,8 @@ class KvCache:
         table = np.ascontiguousarray(table, dtype=np.int32)
         lengths = np.ascontiguousarray(lengths, dtype=np.int32)
         spare = np.ascontiguousarray(spare, dtype=np.int32)
+        if table.ndim != 2 or any(len(a) != parents.size for a in (table, lengths.ravel(), spare.ravel())):
+            raise SptError(ERR_DIMENSIONS, f"expected tables, lengths and spare pages of {parents.size} sequences")
         new_table, new_lengths = np.empty_like(table), np.empty_like(lengths)
         copied = np.empty(batch * beams, np.uint8)
         self.ctx.check(lib().spt_kv_reorder(self.ctx._h, self._h, batch, beams, table.shape[-1], _p(parents), beams,
