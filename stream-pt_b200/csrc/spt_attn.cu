@@ -589,7 +589,10 @@ cudaError_t launch_attention(const AttnArgs &args, cudaStream_t stream) {
   // 198, 128 rows 226 : 183; dim 128, f32, 32 rows 190 : 236, 64 rows 362 : 237;
   // bf16 64 rows 234 : 231, 128 rows 446 : 211.
   const int64_t few = a.type == kKvF32 && a.c.nb > 2 ? 32 : 64;
-  if (a.r.offsets && a.r.tokens * a.group > few * a.r.sequences) return launch_attention_mma(a, stream);
+  if (a.r.offsets && a.r.tokens * a.group > few * a.r.sequences) {
+    const cudaError_t e = launch_attention_mma(a, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
   switch (a.type) {
     case kKvF32: return launch_dims<float>(a, stream);
     case kKvF16: return launch_dims<__half>(a, stream);

@@ -871,14 +871,15 @@ cudaError_t launch(const AttnArgs &a, cudaStream_t stream) {
   using T = MmaTile<NB, IO>;
   cudaError_t e = opt_in_smem(k_attn_mma<NB, IO>, T::kSmem);
   if (e != cudaSuccess) return e;
-  // the register split waits for ever where the block was launched with fewer
+  // the register split waits for ever where the block was launched with fewer:
+  // another compiler's build is left to the kernel for few rows
   static std::atomic<int> regs{0};
   if (regs.load() == 0) {
     cudaFuncAttributes at;
     if ((e = cudaFuncGetAttributes(&at, k_attn_mma<NB, IO>)) != cudaSuccess) return e;
     regs.store(at.numRegs);
   }
-  if (regs.load() != T::kLaunchRegs) return cudaErrorInvalidConfiguration;
+  if (regs.load() != T::kLaunchRegs) return cudaErrorNotSupported;
   return launch_pdl(k_attn_mma<NB, IO>, dim3(a.sm_count), dim3(T::kThreads), T::kSmem, stream, a);
 }
 

@@ -125,7 +125,8 @@ struct AttnArgs {
   int sm_count = 148;
 };
 cudaError_t launch_attention(const AttnArgs &a, cudaStream_t stream);
-// The kernel for many rows of a key head (spt_attn_mma.cu), which launch_attention picks.
+// The kernel for many rows of a key head (spt_attn_mma.cu), which launch_attention
+// picks; cudaErrorNotSupported where it was built with other registers than it needs.
 cudaError_t launch_attention_mma(const AttnArgs &a, cudaStream_t stream);
 size_t attn_mma_workspace_bytes(int sm_count, int nb);
 size_t attn_workspace_bytes(int sm_count, int nb);
