@@ -582,13 +582,17 @@ cudaError_t launch_attention(const AttnArgs &args, cudaStream_t stream) {
   const int size = a.type == kKvF32 ? 4 : 2;
   a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * size)) & 15) == 0;
   a.out_vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * size)) & 15) == 0;
-  // Query rows a sequence and key head, on average, from which the tensor cores'
-  // 128-row tiles pay although most of a tile may be empty.  16 sequences of
-  // 8,000 keys, 8 key heads, this kernel against those tiles, us: dim 64, f32,
-  // 32 rows 93 : 208, 64 rows 175 : 202, 128 rows 334 : 188; bf16 64 rows 122 :
-  // 198, 128 rows 226 : 183; dim 128, f32, 32 rows 190 : 236, 64 rows 362 : 237;
-  // bf16 64 rows 234 : 231, 128 rows 446 : 211.
-  const int64_t few = a.type == kKvF32 && a.c.nb > 2 ? 32 : 64;
+  // Query rows a sequence and key head, on average over the call, from which the
+  // tensor cores' 128-row tiles pay although most of a tile may be empty.  16
+  // sequences of 8,000 keys, 8 key heads, this kernel against those tiles, us: dim
+  // 64, f32, 32 rows 96 : 219, 64 rows 180 : 216, 128 rows 343 : 185; bf16 64 rows
+  // 169 : 215, 128 rows 322 : 180; dim 128, f32, 32 rows 194 : 235, 64 rows 367 :
+  // 239; bf16 32 rows 162 : 238, 64 rows 305 : 239.  A batch of both kinds has one of
+  // them in the wrong kernel: 60 single tokens on 8,000 keys each beside 512 rows
+  // on 2,000 take 882 us there and would take 449 here, 300 single tokens on 2,000
+  // beside a prompt of 2,000 take 1,695 here and would take 1,382 there; in two calls
+  // these are 181 and 318.
+  const int64_t few = a.c.nb > 2 ? 32 : 64;
   if (a.r.offsets && a.r.tokens * a.group > few * a.r.sequences) {
     const cudaError_t e = launch_attention_mma(a, stream);
     if (e != cudaErrorNotSupported) return e;
