@@ -17,7 +17,11 @@ constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kAttnStages = 3;
 constexpr int kAttnCtasPerSm = 2;
 constexpr int kAttnMinTiles = 12;    // a CTA's smallest share: a tile for each warp
-constexpr int kAttnHead = 4;         // an item's beginning and end, in tiles' time
+// An item's beginning and end, in tiles' time.  One f32 token on 2,047 keys, 64 f32
+// and 64 bf16 sequences of up to 8,192 keys, 48 of a window of 128, us: at 1 17.0,
+// 88.0, 91.2, 20.5; at 4 13.1, 87.2, 90.5, 19.1; at 8 14.6, 85.9, 89.1, 19.2; at 16
+// 12.5, 84.5, 87.5, 19.3.
+constexpr int kAttnHead = 4;
 
 // D (16 x 8, f32) += A (16 x 16, f16) * B (16 x 8, f16)
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -43,13 +47,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // of each 32-dim block before their split into f16 terms.  S's fragment is
 // the layout that P^T's operand needs.
 //
-// Bound by instructions: 64 f32 sequences of 8,192 tokens, 8 heads of 64 dims
-// and 8 queries each, read 187 MB in 87 us (2.1 TB/s, 0.55 instructions a clock,
-// the ALU 46% busy with codes becoming f16); one bf16 sequence of 131,000 tokens
-// and 128 dims 151 MB in 70 us (2.1 TB/s).  Three CTAs an SM of steps of two
-// tiles took 110 us instead of 87, steps of two tiles on two CTAs 92; at 128 dims
-// two CTAs an SM took 18% longer than one.  16-bit rows: one f16 term of the weights
-// instead of two took 82 us instead of 88 at 64 dims, 65 instead of 70 at 128.
+// Bound by instructions and the latency of one behind another, as neither issue
+// slots nor a pipe are full and there are 4 warps a scheduler (2 at 128 dims) to
+// change between: 64 f32 sequences of up to 8,192 tokens, 8 heads of 64 dims and 8
+// queries each, read 187 MB in 87 us (2.1 TB/s, 0.55 instructions a clock, the ALU
+// 46% busy with codes becoming f16); 64 such bf16 sequences take 90 us, one bf16
+// sequence of 131,000 tokens and 128 dims 72 us for 151 MB (2.1 TB/s, 0.45
+// instructions a clock).  Three CTAs an SM of steps of two tiles took 110 us
+// instead of 87, steps of two tiles on two CTAs 92; at 128 dims two CTAs an SM took
+// 18% longer than one.  What exactness and safety cost bf16 rows of 64 and of 128
+// dims: the weights' second f16 term 82 -> 88 us and 65 -> 70, scales by what each
+// row sees and waits that are looked at 88 -> 90 and 70 -> 72.
 template <int NB, typename IO, int NT>
 struct Attn {
   static constexpr int kTerms = sizeof(IO) == 4 ? 2 : 1;

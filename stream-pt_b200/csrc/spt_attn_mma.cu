@@ -26,13 +26,20 @@
 // buffered, so that the next tile's products run under a tile's softmax.
 //
 // Bound, for 256 rows x 64 keys at head_dim 64: 1,024 clocks of exponentials
-// (16 a clock on an SM), 1,584 of MMA for f32 rows (48 of 33 clocks) and 1,056
-// for 16-bit rows.  A tile takes 3,300 clocks (f32) or 3,000 (16 bits), those of
-// the softmax warps' own chain: 200 to wait, 350 to fetch S, 300 for its maximum,
-// 1,650 for the weights, 650 to add O, two warps a scheduler.  A prompt of 2,000
-// f32 rows (64 heads on 8 of 64 dims) takes 160 us, tensor cores 32% busy; f16
-// chunks of 12 sequences, 3,000 tokens each, 225 us.  Maxima of three instead of
-// two, or each MMA's S right behind its own O, changed neither by 1%.
+// (16 a clock on an SM), 1,584 of MMA for f32 rows (48 of 33 clocks) and 1,320
+// for 16-bit rows (40).  A tile takes some 3,300 clocks, those of the softmax
+// warps' own chain: 200 to wait, 350 to fetch S, 300 for its maximum, 1,650 for the
+// weights, 650 to add O, two warps a scheduler.  A prompt of 2,000 f32 rows (64
+// heads on 8 of 64 dims) takes 161 us, tensor cores active in 28% of the cycles;
+// f16 chunks of 12 sequences, 3,000 tokens each, 231 us.  Maxima of three instead
+// of two, or each MMA's S right behind its own O, changed neither by 1%.
+//
+// The four roles' code together strains the instruction caches (0.6 to 0.8 warps
+// an issue stall for want of an instruction), so that a few instructions more in
+// one role can cost another 5%: the same change to the loader left prompts of 64
+// dims alone and took f16 ones of 128 dims from 157 to 167 us.  Every instance
+// spills 276 to 320 bytes a thread; the local loads and stores are 0.2 to 0.4% of
+// the instructions executed.
 #include "spt_attn.cuh"
 
 namespace spt {
